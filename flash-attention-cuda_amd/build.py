@@ -44,6 +44,8 @@ HIP_UNITS = [
     ("decode", "decode.hip", []),
     ("kv_cache", "kv_cache.hip", []),
     ("legacy", "legacy.hip", []),
+    ("rope", "rope.hip", []),
+    ("paged", "paged.hip", []),
 ]
 LIB_NAME = "libflashattn_hip.so"
 ARCH = os.environ.get("FA_OFFLOAD_ARCH", "gfx950")

@@ -292,6 +292,222 @@ void append_kv(const at::Tensor &k_cache, const at::Tensor &v_cache, const at::T
                                static_cast<int>(k_cache.size(3)), stream_of(k_cache)));
 }
 
+// ---- rotary positions and the paged cache (no reference counterpart) -------------
+// Tensors of these entry points may be fp16 or bf16, and inputs may be strided
+// (slices of one projection, transposed views) as long as a head's dims are
+// contiguous and every row starts on 16 bytes.
+
+int dtype_of(const at::Tensor &t, const char *name) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK(t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16, name,
+              " must be fp16 or bf16 (got ", t.scalar_type(), ")");
+  return t.scalar_type() == at::kHalf ? FA_F16 : FA_BF16;
+}
+
+void check_head_size(const at::Tensor &t, const char *name) {
+  TORCH_CHECK(t.size(-1) == kHeadDim || t.size(-1) == 128, name, " must have head_dim == ",
+              kHeadDim, " (or 128), got ", t.size(-1));
+}
+
+// Strides of the leading dims (all but the last) are multiples of 8 elements; a
+// dim of size 1 or 0 has no stride that matters.
+void check_strided(const at::Tensor &t, const char *name) {
+  bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
+  for (int64_t d = 0; d + 1 < t.dim(); ++d) ok = ok && (t.size(d) <= 1 || t.stride(d) % 8 == 0);
+  TORCH_CHECK(ok, name, " must have contiguous rows of head_dim elements that start on 16 bytes, "
+              "got strides ", t.strides());
+}
+int64_t stride_of(const at::Tensor &t, int64_t d) { return t.size(d) <= 1 ? 0 : t.stride(d); }
+
+void check_indices(const at::Tensor &t, const char *name, int64_t dim) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK(t.scalar_type() == at::kInt, name, " must be int32 (got ", t.scalar_type(), ")");
+  TORCH_CHECK(t.is_contiguous(), name, " must be contiguous row-major");
+  TORCH_CHECK(t.dim() == dim, name, " must be ", dim, "-D, got ", t.dim(), "-D");
+}
+
+void check_inv_freq(const at::Tensor &inv_freq, int64_t head_dim) {
+  TORCH_CHECK(inv_freq.is_cuda(), "inv_freq must be a CUDA tensor");
+  TORCH_CHECK(inv_freq.scalar_type() == at::kDouble, "inv_freq must be float64 (got ",
+              inv_freq.scalar_type(), ")");
+  TORCH_CHECK(inv_freq.dim() == 1 && inv_freq.is_contiguous(),
+              "inv_freq must be 1-D and contiguous, got ", inv_freq.sizes());
+  const int64_t n = inv_freq.size(0);
+  TORCH_CHECK(n >= 8 && n % 8 == 0 && 2 * n <= head_dim,
+              "inv_freq must hold a multiple of 8 frequencies, at most head_dim / 2, got ", n);
+}
+
+at::Tensor rope_impl(const at::Tensor &x, const char *name, const at::Tensor &positions,
+                     const at::Tensor &inv_freq, bool interleaved, double factor, bool backward) {
+  const int dtype = dtype_of(x, name);
+  TORCH_CHECK(x.dim() == 4, name, " must be 4-D (B, H, N, ", kHeadDim, "), got ", x.dim(), "-D");
+  check_head_size(x, name);
+  check_strided(x, name);
+  TORCH_CHECK(positions.dim() == 1 || positions.dim() == 2,
+              "positions must be [N] or [B, N], got ", positions.sizes());
+  check_indices(positions, "positions", positions.dim());
+  TORCH_CHECK(positions.size(-1) == x.size(2) &&
+                  (positions.dim() == 1 || positions.size(0) == x.size(0)),
+              "positions must be [N] or [B, N] of ", name, ", got ", positions.sizes(), " for ",
+              x.sizes());
+  check_inv_freq(inv_freq, x.size(3));
+  TORCH_CHECK(std::isfinite(factor), "factor must be finite");
+  TORCH_CHECK(x.device() == positions.device() && x.device() == inv_freq.device(), name,
+              ", positions and inv_freq must live on the same device");
+  const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+  at::Tensor out = at::empty(x.sizes(), x.options());
+  if (x.numel() == 0) return out;
+  TORCH_CHECK(x.size(0) <= INT32_MAX && x.size(1) <= INT32_MAX && x.size(2) <= INT32_MAX, name,
+              " is too large");
+  check_status(fa_rope(x.const_data_ptr(), out.data_ptr(), positions.const_data_ptr<int32_t>(),
+                       inv_freq.const_data_ptr<double>(), dtype, static_cast<int>(x.size(0)),
+                       static_cast<int>(x.size(1)), static_cast<int>(x.size(2)),
+                       static_cast<int>(x.size(3)), stride_of(x, 0), stride_of(x, 1),
+                       stride_of(x, 2), positions.dim() == 1 ? 0 : x.size(2),
+                       static_cast<int>(2 * inv_freq.size(0)), interleaved ? 1 : 0,
+                       static_cast<float>(factor), backward ? 1 : 0, stream_of(x)));
+  return out;
+}
+
+at::Tensor rope(const at::Tensor &x, const at::Tensor &positions, const at::Tensor &inv_freq,
+                bool interleaved, double factor) {
+  return rope_impl(x, "x", positions, inv_freq, interleaved, factor, false);
+}
+
+at::Tensor rope_backward(const at::Tensor &grad, const at::Tensor &positions,
+                         const at::Tensor &inv_freq, bool interleaved, double factor) {
+  return rope_impl(grad, "grad", positions, inv_freq, interleaved, factor, true);
+}
+
+// Checks a packed [T, heads, head_dim] input against the cache's type and size.
+fa_rows rows_of(const at::Tensor &t, const char *name, const at::Tensor &k_pages) {
+  dtype_of(t, name);
+  TORCH_CHECK(t.dim() == 3, name, " must be 3-D (T, heads, head_dim), got ", t.dim(), "-D");
+  TORCH_CHECK(t.scalar_type() == k_pages.scalar_type() && t.size(2) == k_pages.size(3), name,
+              " and the pages must have the same type and head_dim, got ", t.scalar_type(), " ",
+              t.sizes(), " and ", k_pages.scalar_type(), " ", k_pages.sizes());
+  check_strided(t, name);
+  return fa_rows{t.const_data_ptr(), stride_of(t, 0), stride_of(t, 1)};
+}
+
+fa_paged paged_of(const at::Tensor &k_pages, const at::Tensor &v_pages,
+                  const at::Tensor &page_table, const at::Tensor &seq_lens,
+                  const at::Tensor &cu_tokens, int64_t tokens) {
+  fa_paged c = {};
+  c.dtype = dtype_of(k_pages, "k_pages");
+  dtype_of(v_pages, "v_pages");
+  TORCH_CHECK(k_pages.dim() == 4, "k_pages must be 4-D (P, H_kv, page_size, head_dim), got ",
+              k_pages.dim(), "-D");
+  TORCH_CHECK(k_pages.sizes() == v_pages.sizes() && k_pages.scalar_type() == v_pages.scalar_type(),
+              "k_pages and v_pages must have identical shapes and types, got ", k_pages.sizes(),
+              " and ", v_pages.sizes());
+  TORCH_CHECK(k_pages.is_contiguous() && v_pages.is_contiguous(),
+              "k_pages and v_pages must be contiguous row-major");
+  check_head_size(k_pages, "k_pages");
+  const int64_t page = k_pages.size(2);
+  TORCH_CHECK(page >= 16 && page <= 1024 && (page & (page - 1)) == 0,
+              "page_size must be a power of two in [16, 1024], got ", page);
+  TORCH_CHECK(k_pages.size(0) > 0 && k_pages.size(1) > 0,
+              "k_pages must hold at least one page and one K/V head, got ", k_pages.sizes());
+  check_indices(page_table, "page_table", 2);
+  check_indices(seq_lens, "seq_lens", 1);
+  check_indices(cu_tokens, "cu_tokens", 1);
+  const int64_t batch = seq_lens.size(0);
+  TORCH_CHECK(page_table.size(0) == batch && cu_tokens.size(0) == batch + 1,
+              "page_table must be [B, max_pages], seq_lens [B] and cu_tokens [B + 1], got ",
+              page_table.sizes(), ", ", seq_lens.sizes(), " and ", cu_tokens.sizes());
+  TORCH_CHECK(batch > 0 && page_table.size(1) > 0,
+              "page_table must hold at least one sequence and one page, got ",
+              page_table.sizes());
+  TORCH_CHECK(k_pages.device() == v_pages.device() && k_pages.device() == page_table.device() &&
+                  k_pages.device() == seq_lens.device() && k_pages.device() == cu_tokens.device(),
+              "pages, page_table, seq_lens and cu_tokens must live on the same device");
+  TORCH_CHECK(k_pages.size(0) <= INT32_MAX && k_pages.size(1) <= INT32_MAX &&
+                  batch <= INT32_MAX && page_table.size(1) <= INT32_MAX && tokens <= INT32_MAX,
+              "pages, page_table or packed tokens too large");
+  c.k_pages = k_pages.data_ptr();
+  c.v_pages = v_pages.data_ptr();
+  c.page_table = page_table.const_data_ptr<int32_t>();
+  c.seq_lens = seq_lens.const_data_ptr<int32_t>();
+  c.cu_tokens = cu_tokens.const_data_ptr<int32_t>();
+  c.batch = static_cast<int>(batch);
+  c.tokens = static_cast<int>(tokens);
+  c.kv_heads = static_cast<int>(k_pages.size(1));
+  c.head_dim = static_cast<int>(k_pages.size(3));
+  c.page_size = static_cast<int>(page);
+  c.num_pages = static_cast<int>(k_pages.size(0));
+  c.max_pages = static_cast<int>(page_table.size(1));
+  return c;
+}
+
+void check_query_heads(const at::Tensor &q, const at::Tensor &k_pages) {
+  const int64_t heads = q.size(1), kv_heads = k_pages.size(1);
+  TORCH_CHECK(heads > 0 && heads <= INT32_MAX && heads % kv_heads == 0 && heads / kv_heads <= 128,
+              "the K/V head count must divide the query head count, into groups of at most 128, "
+              "got H=", heads, " H_kv=", kv_heads);
+}
+
+c10::optional<at::Tensor> append_paged(const at::Tensor &k_pages, const at::Tensor &v_pages,
+                                       const at::Tensor &k, const at::Tensor &v,
+                                       const at::Tensor &page_table, const at::Tensor &seq_lens,
+                                       const at::Tensor &cu_tokens,
+                                       const c10::optional<at::Tensor> &q,
+                                       const c10::optional<at::Tensor> &inv_freq,
+                                       bool interleaved, double factor) {
+  TORCH_CHECK(q.has_value() == inv_freq.has_value(),
+              "append_paged takes q and inv_freq together or neither");
+  TORCH_CHECK(k.dim() == 3, "k must be 3-D (T, heads, head_dim), got ", k.dim(), "-D");
+  const fa_paged cache = paged_of(k_pages, v_pages, page_table, seq_lens, cu_tokens, k.size(0));
+  const fa_rows kr = rows_of(k, "k", k_pages), vr = rows_of(v, "v", k_pages);
+  TORCH_CHECK(k.sizes() == v.sizes() && k.size(1) == k_pages.size(1),
+              "append_paged expects k and v of shape [T, H_kv, head_dim] matching the pages, got k=",
+              k.sizes(), " v=", v.sizes(), " pages=", k_pages.sizes());
+  TORCH_CHECK(k_pages.device() == k.device() && k_pages.device() == v.device(),
+              "pages, k and v must live on the same device");
+  fa_rows qr = {};
+  if (q.has_value()) {
+    qr = rows_of(*q, "q", k_pages);
+    TORCH_CHECK(q->size(0) == k.size(0), "q, k and v must have the same number of tokens, got ",
+                q->size(0), " and ", k.size(0));
+    check_query_heads(*q, k_pages);
+    check_inv_freq(*inv_freq, k_pages.size(3));
+    TORCH_CHECK(std::isfinite(factor), "factor must be finite");
+    TORCH_CHECK(k_pages.device() == q->device() && k_pages.device() == inv_freq->device(),
+                "pages, q and inv_freq must live on the same device");
+  }
+  const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(k_pages.device());
+  c10::optional<at::Tensor> out;
+  if (q.has_value()) out = at::empty(q->sizes(), q->options());
+  if (k.size(0) == 0) return out;
+  check_status(fa_append_paged(
+      &cache, &kr, &vr, q.has_value() ? &qr : nullptr, out.has_value() ? out->data_ptr() : nullptr,
+      q.has_value() ? static_cast<int>(q->size(1)) : 0,
+      q.has_value() ? inv_freq->const_data_ptr<double>() : nullptr,
+      q.has_value() ? static_cast<int>(2 * inv_freq->size(0)) : 0, interleaved ? 1 : 0,
+      static_cast<float>(factor), stream_of(k_pages)));
+  return out;
+}
+
+at::Tensor attend_paged(const at::Tensor &q, const at::Tensor &k_pages, const at::Tensor &v_pages,
+                        const at::Tensor &page_table, const at::Tensor &seq_lens,
+                        const at::Tensor &cu_tokens, double scale) {
+  TORCH_CHECK(q.dim() == 3, "q must be 3-D (T, heads, head_dim), got ", q.dim(), "-D");
+  const fa_paged cache = paged_of(k_pages, v_pages, page_table, seq_lens, cu_tokens, q.size(0));
+  const fa_rows qr = rows_of(q, "q", k_pages);
+  check_query_heads(q, k_pages);
+  TORCH_CHECK(q.device() == k_pages.device(), "q and the pages must live on the same device");
+  TORCH_CHECK(std::isfinite(scale), "scale must be finite");
+  const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(q.device());
+  at::Tensor o = at::empty(q.sizes(), q.options());
+  if (q.size(0) == 0) return o;
+  const size_t ws_bytes = fa_attend_paged_workspace_bytes(
+      cache.tokens, static_cast<int>(q.size(1)), cache.kv_heads, cache.head_dim);
+  const Workspace ws(ws_bytes);
+  check_status(fa_attend_paged(&cache, &qr, o.data_ptr(), static_cast<int>(q.size(1)),
+                               static_cast<float>(scale), ws.ptr, ws_bytes, stream_of(q)));
+  return o;
+}
+
 // bindings.cpp:80-97.
 py::list occupancy_report() {
   // The first call counts the rows, the second fills them.
@@ -416,6 +632,23 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("_decode_gqa_fp32", &decode_gqa_fp32, py::arg("q"), py::arg("k_cache"),
         py::arg("v_cache"), py::arg("seq_lens"), py::arg("scale"),
         py::arg("split_size") = 0);
+
+  // Rotary positions and the paged cache (no reference counterpart).
+  m.def("rope", &rope, "Rotary positions of [B, H, N, D] queries or keys", py::arg("x"),
+        py::arg("positions"), py::arg("inv_freq"), py::arg("interleaved") = false,
+        py::arg("factor") = 1.0);
+  m.def("rope_backward", &rope_backward, "Gradient of rope with respect to x", py::arg("grad"),
+        py::arg("positions"), py::arg("inv_freq"), py::arg("interleaved") = false,
+        py::arg("factor") = 1.0);
+  m.def("append_paged", &append_paged,
+        "Write a ragged batch's new K/V into their pages, rotated with q when inv_freq is given",
+        py::arg("k_pages"), py::arg("v_pages"), py::arg("k"), py::arg("v"), py::arg("page_table"),
+        py::arg("seq_lens"), py::arg("cu_tokens"), py::arg("q") = py::none(),
+        py::arg("inv_freq") = py::none(), py::arg("interleaved") = false, py::arg("factor") = 1.0);
+  m.def("attend_paged", &attend_paged,
+        "Causal attention of a ragged batch's new tokens over a paged KV cache", py::arg("q"),
+        py::arg("k_pages"), py::arg("v_pages"), py::arg("page_table"), py::arg("seq_lens"),
+        py::arg("cu_tokens"), py::arg("scale"));
 
   // bindings.cpp:131-133: the v1 kernels, (N, 64) fp32, one head, no mask.
   m.def("legacy_naive", &legacy_naive, "v1 naive kernel (N, 64) fp32");

@@ -89,6 +89,47 @@ int launch_kv_append(void *k_cache, void *v_cache, const void *k_new, const void
 int launch_legacy_attention(const float *q, const float *k, const float *v, float *o, int n,
                             int variant, hipStream_t stream);
 
+// Rotary positions (rope.hip): out is contiguous [B, H, N, D]; strides of x in
+// elements; pos_batch 0 shares one row of positions.
+int launch_rope(const void *x, void *out, const int32_t *positions, const double *inv_freq,
+                bool bf16, int batch, int heads, int seq, int head_dim, int64_t x_batch,
+                int64_t x_head, int64_t x_row, int64_t pos_batch, int rotary, bool interleaved,
+                float factor, bool backward, hipStream_t stream);
+
+// A paged batch's new tokens into their pages (rope.hip), queries and keys turned
+// when rotary > 0. q_heads 0: no queries.
+struct AppendPagedParams {
+  const void *q, *k, *v;  // packed [tokens, heads, D] with the strides below
+  void *q_out;            // contiguous [tokens, q_heads, D]
+  void *k_pages, *v_pages;
+  const int32_t *page_table, *seq_lens, *cu_tokens;
+  const double *inv_freq;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+  int batch, tokens, q_heads, kv_heads, head_dim, num_pages, page_shift, max_pages, rotary;
+  int heads_per_thread;   // set by the launcher
+  float factor;
+  bool interleaved;
+};
+int launch_append_paged(AppendPagedParams p, bool bf16, hipStream_t stream);
+
+// Attention of packed new tokens over a paged cache (paged.hip).
+struct AttendPagedParams {
+  const void *q, *k_pages, *v_pages;
+  const int32_t *page_table, *seq_lens, *cu_tokens;
+  void *out;              // contiguous [tokens, heads, D]
+  int64_t q_token, q_head;
+  int batch, tokens, heads, kv_heads, num_pages, page_shift, max_pages;
+  // Set by the launcher.
+  int group, slot_rows, capacity;
+  float c;
+  bool negate;
+  void *records;
+  float *partials;
+};
+size_t attend_paged_workspace_bytes(int tokens, int group, int head_dim);
+int launch_attend_paged(AttendPagedParams p, bool bf16, int head_dim, float scale, void *workspace,
+                        hipStream_t stream);
+
 // Occupancy rows for each kernel (appended to `out`, at most `cap` rows).
 int prefill_occupancy(fa_occupancy_entry *out, int cap, int *n);
 int decode_occupancy(fa_occupancy_entry *out, int cap, int *n);

@@ -456,6 +456,211 @@ int fa_kv_append_hd(void *k_cache, void *v_cache, const void *k_new, const void 
                         head_dim, stream);
 }
 
+namespace {
+bool multiple_of_8(int64_t x) { return x % 8 == 0; }
+
+int check_dtype(int dtype) {
+  if (dtype != FA_F16 && dtype != FA_BF16)
+    return set_error(FA_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+  return FA_OK;
+}
+
+int check_rotation(const double *inv_freq, int rotary_dim, int head_dim, float factor) {
+  if (rotary_dim < 16 || rotary_dim > head_dim || rotary_dim % 16 != 0)
+    return set_error(FA_ERR_INVALID_ARGUMENT,
+                     "rotary_dim must be a multiple of 16 in [16, head_dim], got %d", rotary_dim);
+  if (inv_freq == nullptr || (reinterpret_cast<uintptr_t>(inv_freq) & 7u) != 0)
+    return set_error(FA_ERR_INVALID_ARGUMENT, "inv_freq must be non-NULL and 8-byte aligned");
+  if (!std::isfinite(factor))
+    return set_error(FA_ERR_INVALID_ARGUMENT, "factor must be finite");
+  return FA_OK;
+}
+
+int check_rows(const fa_rows *r, const char *name) {
+  if (r == nullptr || r->data == nullptr)
+    return set_error(FA_ERR_INVALID_ARGUMENT, "%s must be non-NULL", name);
+  if (!aligned16(r->data) || !multiple_of_8(r->token_stride) || !multiple_of_8(r->head_stride))
+    return set_error(FA_ERR_INVALID_ARGUMENT,
+                     "%s must be 16-byte aligned with strides that are multiples of 8", name);
+  return FA_OK;
+}
+
+// Checks a cache description; *page_shift gets log2 of its page size.
+int check_paged(const fa_paged *c, int *page_shift) {
+  if (c == nullptr) return set_error(FA_ERR_INVALID_ARGUMENT, "cache must be non-NULL");
+  int rc = check_dtype(c->dtype);
+  if (rc == FA_OK) rc = check_head_dim(c->head_dim);
+  if (rc != FA_OK) return rc;
+  if (c->k_pages == nullptr || c->v_pages == nullptr || c->page_table == nullptr ||
+      c->seq_lens == nullptr || c->cu_tokens == nullptr)
+    return set_error(FA_ERR_INVALID_ARGUMENT,
+                     "k_pages, v_pages, page_table, seq_lens and cu_tokens must be non-NULL");
+  if (!aligned16(c->k_pages) || !aligned16(c->v_pages))
+    return set_error(FA_ERR_INVALID_ARGUMENT, "k_pages and v_pages must be 16-byte aligned");
+  if (((reinterpret_cast<uintptr_t>(c->page_table) | reinterpret_cast<uintptr_t>(c->seq_lens) |
+        reinterpret_cast<uintptr_t>(c->cu_tokens)) & 3u) != 0)
+    return set_error(FA_ERR_INVALID_ARGUMENT,
+                     "page_table, seq_lens and cu_tokens must be 4-byte aligned");
+  if (c->batch <= 0 || c->tokens <= 0 || c->kv_heads <= 0 || c->num_pages <= 0 ||
+      c->max_pages <= 0)
+    return set_error(FA_ERR_INVALID_ARGUMENT,
+                     "batch, tokens, kv_heads, num_pages and max_pages must be > 0, got %d, %d, "
+                     "%d, %d and %d", c->batch, c->tokens, c->kv_heads, c->num_pages,
+                     c->max_pages);
+  if (c->page_size < 16 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)) != 0)
+    return set_error(FA_ERR_INVALID_ARGUMENT,
+                     "page_size must be a power of two in [16, 1024], got %d", c->page_size);
+  if (static_cast<int64_t>(c->max_pages) * c->page_size > kMaxCacheRows)
+    return set_error(FA_ERR_INVALID_ARGUMENT, "max_pages * page_size must be at most %d, got %lld",
+                     kMaxCacheRows, static_cast<long long>(c->max_pages) * c->page_size);
+  // Threads of the append's grid, and row indices of the attention, stay in int.
+  if (c->tokens > (1 << 24))
+    return set_error(FA_ERR_INVALID_ARGUMENT, "at most 2^24 packed tokens, got %d", c->tokens);
+  if (c->kv_heads > 8192)
+    return set_error(FA_ERR_INVALID_ARGUMENT, "at most 8192 K/V heads, got %d", c->kv_heads);
+  *page_shift = __builtin_ctz(static_cast<unsigned>(c->page_size));
+  return FA_OK;
+}
+
+int check_query_groups(int heads, int kv_heads) {
+  const int rc = check_groups(heads, kv_heads);
+  if (rc != FA_OK) return rc;
+  if (heads / kv_heads > 128)
+    return set_error(FA_ERR_INVALID_ARGUMENT,
+                     "at most 128 query heads per K/V head, got H=%d H_kv=%d", heads, kv_heads);
+  return FA_OK;
+}
+}  // namespace
+
+int fa_rope(const void *x, void *out, const int32_t *positions, const double *inv_freq, int dtype,
+            int batch, int heads, int seq, int head_dim, int64_t x_batch_stride,
+            int64_t x_head_stride, int64_t x_row_stride, int64_t positions_batch_stride,
+            int rotary_dim, int interleaved, float factor, int backward, void *stream) {
+  clear_error();
+  int rc = check_dtype(dtype);
+  if (rc == FA_OK) rc = check_head_dim(head_dim);
+  if (rc == FA_OK) rc = check_rotation(inv_freq, rotary_dim, head_dim, factor);
+  if (rc != FA_OK) return rc;
+  if (x == nullptr || out == nullptr || positions == nullptr)
+    return set_error(FA_ERR_INVALID_ARGUMENT, "x, out and positions must be non-NULL");
+  if (!aligned16(x) || !aligned16(out) || !multiple_of_8(x_batch_stride) ||
+      !multiple_of_8(x_head_stride) || !multiple_of_8(x_row_stride))
+    return set_error(FA_ERR_INVALID_ARGUMENT,
+                     "x and out must be 16-byte aligned and x's strides multiples of 8");
+  if ((reinterpret_cast<uintptr_t>(positions) & 3u) != 0)
+    return set_error(FA_ERR_INVALID_ARGUMENT, "positions must be 4-byte aligned");
+  if (batch <= 0 || heads <= 0 || seq <= 0)
+    return set_error(FA_ERR_INVALID_ARGUMENT, "batch, heads and seq must be > 0, got %d, %d, %d",
+                     batch, heads, seq);
+  if (heads > 65535 ||
+      static_cast<int64_t>(batch) * seq * (head_dim / 16) > 0x7fffffffll)
+    return set_error(FA_ERR_INVALID_ARGUMENT, "batch * seq or heads too large");
+  return launch_rope(x, out, positions, inv_freq, dtype == FA_BF16, batch, heads, seq, head_dim,
+                     x_batch_stride, x_head_stride, x_row_stride, positions_batch_stride,
+                     rotary_dim, interleaved != 0, factor, backward != 0,
+                     static_cast<hipStream_t>(stream));
+}
+
+int fa_append_paged(const fa_paged *cache, const fa_rows *k, const fa_rows *v, const fa_rows *q,
+                    void *q_out, int heads, const double *inv_freq, int rotary_dim,
+                    int interleaved, float factor, void *stream) {
+  clear_error();
+  int shift = 0;
+  int rc = check_paged(cache, &shift);
+  if (rc == FA_OK) rc = check_rows(k, "k");
+  if (rc == FA_OK) rc = check_rows(v, "v");
+  if (rc != FA_OK) return rc;
+  AppendPagedParams p = {};
+  if (rotary_dim != 0) {
+    rc = check_rotation(inv_freq, rotary_dim, cache->head_dim, factor);
+    if (rc == FA_OK) rc = check_rows(q, "q");
+    if (rc == FA_OK) rc = check_query_groups(heads, cache->kv_heads);
+    if (rc != FA_OK) return rc;
+    if (q_out == nullptr || !aligned16(q_out))
+      return set_error(FA_ERR_INVALID_ARGUMENT, "q_out must be non-NULL and 16-byte aligned");
+    if (heads > 32768) return set_error(FA_ERR_INVALID_ARGUMENT, "at most 32768 heads, got %d", heads);
+    p.q = q->data;
+    p.q_token = q->token_stride;
+    p.q_head = q->head_stride;
+    p.q_out = q_out;
+    p.q_heads = heads;
+    p.inv_freq = inv_freq;
+  }
+  p.k = k->data;
+  p.k_token = k->token_stride;
+  p.k_head = k->head_stride;
+  p.v = v->data;
+  p.v_token = v->token_stride;
+  p.v_head = v->head_stride;
+  p.k_pages = cache->k_pages;
+  p.v_pages = cache->v_pages;
+  p.page_table = cache->page_table;
+  p.seq_lens = cache->seq_lens;
+  p.cu_tokens = cache->cu_tokens;
+  p.batch = cache->batch;
+  p.tokens = cache->tokens;
+  p.kv_heads = cache->kv_heads;
+  p.head_dim = cache->head_dim;
+  p.num_pages = cache->num_pages;
+  p.page_shift = shift;
+  p.max_pages = cache->max_pages;
+  p.rotary = rotary_dim;
+  p.factor = factor;
+  p.interleaved = interleaved != 0;
+  return launch_append_paged(p, cache->dtype == FA_BF16, static_cast<hipStream_t>(stream));
+}
+
+size_t fa_attend_paged_workspace_bytes(int tokens, int heads, int kv_heads, int head_dim) {
+  clear_error();
+  if (tokens <= 0) {
+    set_error(FA_ERR_INVALID_ARGUMENT, "tokens must be > 0, got %d", tokens);
+    return 0;
+  }
+  if (check_head_dim(head_dim) != FA_OK || check_query_groups(heads, kv_heads) != FA_OK) return 0;
+  return attend_paged_workspace_bytes(tokens, heads / kv_heads, head_dim);
+}
+
+int fa_attend_paged(const fa_paged *cache, const fa_rows *q, void *out, int heads, float scale,
+                    void *workspace, size_t workspace_bytes, void *stream) {
+  clear_error();
+  int shift = 0;
+  int rc = check_paged(cache, &shift);
+  if (rc == FA_OK) rc = check_rows(q, "q");
+  if (rc == FA_OK) rc = check_query_groups(heads, cache->kv_heads);
+  if (rc != FA_OK) return rc;
+  if (out == nullptr || !aligned16(out))
+    return set_error(FA_ERR_INVALID_ARGUMENT, "out must be non-NULL and 16-byte aligned");
+  if (!std::isfinite(scale) || !std::isfinite(scale * kLog2e))
+    return set_error(FA_ERR_INVALID_ARGUMENT, "scale must be finite");
+  const size_t need =
+      attend_paged_workspace_bytes(cache->tokens, heads / cache->kv_heads, cache->head_dim);
+  if (need == 0) return set_error(FA_ERR_HIP, "could not query the compute-unit count");
+  if (workspace == nullptr || workspace_bytes < need)
+    return set_error(FA_ERR_WORKSPACE, "attention workspace too small: need %zu bytes, got %zu",
+                     need, workspace == nullptr ? size_t{0} : workspace_bytes);
+  if (!aligned16(workspace))
+    return set_error(FA_ERR_INVALID_ARGUMENT, "workspace must be 16-byte aligned");
+  AttendPagedParams p = {};
+  p.q = q->data;
+  p.q_token = q->token_stride;
+  p.q_head = q->head_stride;
+  p.k_pages = cache->k_pages;
+  p.v_pages = cache->v_pages;
+  p.page_table = cache->page_table;
+  p.seq_lens = cache->seq_lens;
+  p.cu_tokens = cache->cu_tokens;
+  p.out = out;
+  p.batch = cache->batch;
+  p.tokens = cache->tokens;
+  p.heads = heads;
+  p.kv_heads = cache->kv_heads;
+  p.num_pages = cache->num_pages;
+  p.page_shift = shift;
+  p.max_pages = cache->max_pages;
+  return launch_attend_paged(p, cache->dtype == FA_BF16, cache->head_dim, scale, workspace,
+                             static_cast<hipStream_t>(stream));
+}
+
 int fa_legacy_attention(const float *q, const float *k, const float *v, float *o, int n,
                         int variant, void *stream) {
   clear_error();

@@ -21,6 +21,13 @@ cache write before a decode step (row ``seq_lens[b]``, then ``seq_lens[b] +=
 1``, on the device), so a whole append + decode step can be captured in a
 HIP graph and replayed per token.
 
+Also added, for serving over a paged cache (fp16 or bf16, both head sizes):
+``rope`` / ``rope_backward`` (rotary positions and their gradient),
+``rope_frequencies`` (their frequencies, also for stretched contexts),
+``append_paged`` (a ragged batch's new tokens, packed as [T, heads, D], into
+their pages, queries and keys rotated on the way) and ``attend_paged`` (those
+tokens' causal attention over the pages: prompt chunks, single tokens or both).
+
 The v1 ``legacy_naive/tiled/fused`` kernels of the reference (one (N, 64)
 fp32 head, no mask, scale 1/8) are there too, with the reference's checks.
 
@@ -41,6 +48,8 @@ try:
         _prefill_fp32,
         _prefill_gqa_fp32,
         append_kv,
+        append_paged,
+        attend_paged,
         choose_decode_split,
         decode,
         decode_gqa,
@@ -52,6 +61,8 @@ try:
         occupancy_report,
         prefill,
         prefill_gqa,
+        rope,
+        rope_backward,
     )
 except ImportError as exc:  # pragma: no cover - exercised only when unbuilt
     raise ImportError(
@@ -60,6 +71,7 @@ except ImportError as exc:  # pragma: no cover - exercised only when unbuilt
         f"first. Underlying error: {exc}"
     ) from exc
 
+from ._rotary import rope_frequencies  # noqa: E402,F401
 
 __all__ = [
     "prefill",
@@ -67,6 +79,11 @@ __all__ = [
     "prefill_gqa",
     "decode_gqa",
     "append_kv",
+    "rope",
+    "rope_backward",
+    "rope_frequencies",
+    "append_paged",
+    "attend_paged",
     "head_dim",
     "head_dims",
     "occupancy_report",
