@@ -123,7 +123,7 @@ struct AttendPagedParams {
   int group, slot_rows, capacity;
   float c;
   bool negate;
-  void *records;
+  unsigned *counters;
   float *partials;
 };
 size_t attend_paged_workspace_bytes(int tokens, int group, int head_dim);

@@ -20,8 +20,8 @@
 //            that knows the lengths. Each block finds its own share from
 //            seq_lens and cu_tokens.
 //   merge  = an item that a share's border cuts leaves one fp32 partial (O, m,
-//            l) per share in the workspace, and a second launch joins them in
-//            the order of the shares, so results do not depend on timing.
+//            l) per share in the workspace; the block that finishes last joins
+//            them in the order of the shares, so results do not depend on timing.
 //
 // Block: 256 threads, 4 waves, two blocks per CU.
 //   wide item: wave w owns query rows [32 w, +32); the waves share 64-key K and V
@@ -52,7 +52,6 @@ constexpr int kTileKeys = 64;     // keys per tile of a wide item, and the unit 
 constexpr int kWideRows = 128;    // query rows of a wide item
 constexpr int kNarrowRows = 32;   // most query rows of a narrow item
 constexpr int kRingBytes = 64 * 1024;
-constexpr int kMergeRows = 8;     // rows per merge block
 constexpr int kItemKeys = 128;    // an item's fixed cost, in keys
 constexpr int kMinShareKeys = 256;  // least weight of a share
 constexpr int kSnapTiles = 1;     // borders this close to an item's end move there
@@ -137,20 +136,38 @@ __device__ __forceinline__ int64_t weight_before(const AttendPagedParams &p, con
   return tile * each + static_cast<int64_t>(t.tokens) * tile * (tile + 1) / 2;
 }
 
-// A share's border: before key tile `kt` of item (b, kvh, tile).
+// Key tiles of an item.
+__device__ __forceinline__ int key_tiles(int end) { return (end + kTileKeys - 1) / kTileKeys; }
+
+// floor(a / b) for 0 <= a < 2^52, b > 0: a product in fp64 (one estimate off by at
+// most one, then corrected) instead of a 64-bit integer division, which costs
+// over a hundred dependent instructions at the start of every block.
+__device__ __forceinline__ int64_t floor_div(int64_t a, int64_t b) {
+  int64_t q = static_cast<int64_t>(static_cast<double>(a) / static_cast<double>(b));
+  if (q * b > a) --q;
+  if ((q + 1) * b <= a) ++q;
+  return q;
+}
+__device__ __forceinline__ int64_t ceil_div(int64_t a, int64_t b) { return floor_div(a + b - 1, b); }
+
+// A share's border: before key tile `kt` of item (b, kvh, tile); `from` is the weight
+// of the sequences before b.
 struct Border {
   int b, kvh, tile, kt;
+  Seq s;
+  int pad;
+  int64_t from;
 };
-__device__ __forceinline__ bool same_item(const Border &a, const Border &b) {
-  return a.b == b.b && a.kvh == b.kvh && a.tile == b.tile;
-}
 
-// The border at weight `at` inside sequence b (0 <= at < H_kv * whole).
+// The border at weight `at` inside sequence b (0 <= at - from < H_kv * whole).
 __device__ Border border_in(const AttendPagedParams &p, const Seq &s, const Tiles &t, int b,
-                            int64_t whole, int64_t at) {
+                            int64_t whole, int64_t from, int64_t at) {
   Border r;
   r.b = b;
-  r.kvh = static_cast<int>(at / whole);
+  r.s = s;
+  r.from = from;
+  at -= from;
+  r.kvh = static_cast<int>(floor_div(at, whole));
   at -= r.kvh * whole;
   int lo = 0, hi = t.count;  // the last tile whose weight_before is <= at
   while (hi - lo > 1) {
@@ -159,7 +176,7 @@ __device__ Border border_in(const AttendPagedParams &p, const Seq &s, const Tile
     else hi = mid;
   }
   r.tile = lo;
-  const int tiles = (key_end(p, s, t, lo) + kTileKeys - 1) / kTileKeys;
+  const int tiles = key_tiles(key_end(p, s, t, lo));
   const int64_t in = at - weight_before(p, s, t, lo) - kItemKeys;
   r.kt = static_cast<int>(min(max(in, int64_t{0}) / kTileKeys, static_cast<int64_t>(tiles)));
   // A border close to an item's end moves there: a partial costs more than the keys it balances.
@@ -168,14 +185,20 @@ __device__ Border border_in(const AttendPagedParams &p, const Seq &s, const Tile
   return r;
 }
 
-// Record of a share's first border, kept for the merge launch.
-struct Record {
-  Border at;
-  int tiles;   // key tiles of that item
-  int t0, n;   // its packed tokens
-  int pad;
+// The shares that an item of `tiles` key tiles at weights [x0, x1) is cut into: the
+// first border inside it and the number of pieces. Piece i is share
+// first + i - 1's; a border k lies inside when border_in gives it 0 < kt < tiles.
+struct Pieces {
+  int first, count;
 };
-static_assert(sizeof(Record) == 32, "two 16-byte pieces");
+__device__ __forceinline__ Pieces pieces_of(int64_t x0, int64_t x1, int tiles, int64_t share) {
+  Pieces r;
+  r.first = static_cast<int>(ceil_div(x0 + kItemKeys + kSnapTiles * kTileKeys, share));
+  const int64_t stop =
+      min(x1, x0 + kItemKeys + static_cast<int64_t>(tiles - kSnapTiles + 1) * kTileKeys);
+  r.count = static_cast<int>(ceil_div(stop, share)) - r.first + 1;
+  return r;
+}
 
 // ---- a wave's rows -----------------------------------------------------------------
 
@@ -376,9 +399,26 @@ __device__ __forceinline__ void load_slab(const void *pages, int64_t at,
 
 // ---- results -------------------------------------------------------------------------
 
-// Partial of a share: rows of D floats, then (m, l) pairs.
+// Partial of a share. Narrow items: rows of D floats, then (m, l) pairs from slot_rows D
+// on. Wide items: each wave's accumulators as (pair of elements, lane), then the pairs.
 __device__ __forceinline__ float *partial_of(const AttendPagedParams &p, int slot, int head_dim) {
   return p.partials + static_cast<int64_t>(slot) * p.slot_rows * (head_dim + 2);
+}
+
+// Two floats of a partial, for another block: coherent 8-byte stores and loads (mfma_tile.h).
+// They go past the L2, so the lanes of an instruction must cover contiguous memory: with
+// a wide item's rows stored row by row (8 bytes in each of 32 rows per instruction) a
+// prompt of 4096 tokens and 14 heads took 85.6 us, in accumulator order 58.6.
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void publish2(float *p, float x, float y) {
+  const floatx2 a = {x, y};
+  __hip_atomic_store(reinterpret_cast<uint64_t *>(p), __builtin_bit_cast(uint64_t, a),
+                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ floatx2 fetch2(const float *p) {
+  return __builtin_bit_cast(
+      floatx2, __hip_atomic_load(reinterpret_cast<uint64_t *>(const_cast<float *>(p)),
+                                 __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
 
 template <typename T>
@@ -426,6 +466,23 @@ __device__ __forceinline__ void clear_v(unsigned tile, int rows, int from, unsig
       *reinterpret_cast<lds_floatx4 *>(static_cast<uintptr_t>(tile + 16u * i)) = zero;
     }
   }
+}
+
+// Normalises and stores the lane's half of its query row.
+template <typename T, int D>
+__device__ __forceinline__ void write_rows(const AttendPagedParams &p, const Item &it, int row,
+                                           int g, const floatx16 (&o)[D / 32], float l) {
+  if (row >= it.n * p.group) return;
+  const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;  // NaN stays NaN
+  T *out = out_row<T>(p, it.t0, it.kvh, row, D);
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const floatx4 x = {o[i][4 * a] * inv, o[i][4 * a + 1] * inv, o[i][4 * a + 2] * inv,
+                         o[i][4 * a + 3] * inv};
+      store4<T>(out + 32 * i + 8 * a + 4 * g, x);
+    }
 }
 
 template <typename T, int D>
@@ -496,34 +553,53 @@ __device__ __forceinline__ void wide_item(const AttendPagedParams &p, const Item
   }
   block_barrier();  // the ring may be filled for the next item
 
-  if (row >= rows) return;
-  const float l = r.l[0];
+  if (!has_rows) return;
   if (it.slot < 0) {
-    const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;  // NaN stays NaN
-    T *o = out_row<T>(p, it.t0, it.kvh, row, D);
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-      for (int a = 0; a < 4; ++a) {
-        const floatx4 x = {r.o[i][4 * a] * inv, r.o[i][4 * a + 1] * inv, r.o[i][4 * a + 2] * inv,
-                           r.o[i][4 * a + 3] * inv};
-        store4<T>(o + 32 * i + 8 * a + 4 * g, x);
-      }
+    write_rows<T, D>(p, it, row, g, r.o, r.l[0]);
   } else {
-    float *part = partial_of(p, it.slot, D);
+    float *part = partial_of(p, it.slot, D) + wave * (32 * D) + 2 * lane;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-      for (int a = 0; a < 4; ++a) {
-        const floatx4 x = {r.o[i][4 * a], r.o[i][4 * a + 1], r.o[i][4 * a + 2], r.o[i][4 * a + 3]};
-        *reinterpret_cast<floatx4 *>(part + row * D + 32 * i + 8 * a + 4 * g) = x;
-      }
-    if (g == 0) {
-      float *ml = part + p.slot_rows * D + 2 * row;
-      ml[0] = r.m;
-      ml[1] = l;
+      for (int a = 0; a < 8; ++a)
+        publish2(part + (8 * i + a) * 128, r.o[i][2 * a], r.o[i][2 * a + 1]);
+    if (g == 0)
+      publish2(partial_of(p, it.slot, D) + kWideRows * D + 2 * row, r.m, r.l[0]);
+  }
+}
+
+// Joins a wide item's pieces, first to last, and writes its rows.
+template <typename T, int D>
+__device__ __forceinline__ void join_wide(const AttendPagedParams &p, const Item &it,
+                                          const Pieces &pc) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row = 32 * wave + (lane & 31);
+  if (32 * wave >= it.n * p.group) return;
+  float m = -INFINITY, l = 0.f;
+  floatx16 o[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int a = 0; a < 16; ++a) o[i][a] = 0.f;
+  for (int j = 0; j < pc.count; ++j) {
+    const float *part = partial_of(p, 2 * (pc.first + j - 1) + (j == 0 ? 1 : 0), D);
+    const floatx2 ml = fetch2(part + kWideRows * D + 2 * row);
+    floatx2 x[D / 4];
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i) x[i] = fetch2(part + wave * (32 * D) + 128 * i + 2 * lane);
+    const float top = fmaxf(m, ml[0]);
+    const float a = m == -INFINITY ? 0.f : fast_exp2(m - top);
+    const float b = ml[0] == -INFINITY ? 0.f : fast_exp2(ml[0] - top);
+    m = top;
+    l = l * a + ml[1] * b;
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i) {
+      o[i / 8][2 * (i % 8)] = o[i / 8][2 * (i % 8)] * a + x[i][0] * b;
+      o[i / 8][2 * (i % 8) + 1] = o[i / 8][2 * (i % 8) + 1] * a + x[i][1] * b;
     }
   }
+  write_rows<T, D>(p, it, row, lane >> 5, o, l);
 }
 
 template <typename T, int D>
@@ -606,36 +682,72 @@ __device__ __forceinline__ void narrow_item(const AttendPagedParams &p, const It
     }
   }
   block_barrier();
-  for (int i = threadIdx.x; i < rows * (D / 4); i += kThreads) {
-    const int at = i / (D / 4), piece = i % (D / 4);
+  for (int i = threadIdx.x; i < rows * (D / 2); i += kThreads) {
+    const int at = i / (D / 2), pair = i % (D / 2);  // two dims per thread
     float m = -INFINITY, l = 0.f;
     float w[kWaves];
 #pragma unroll
     for (int j = 0; j < kWaves; ++j) m = fmaxf(m, exchange_ml[2 * (j * kNarrowRows + at)]);
-    floatx4 o = {0.f, 0.f, 0.f, 0.f};
+    floatx2 o = {0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < kWaves; ++j) {
       const float mj = exchange_ml[2 * (j * kNarrowRows + at)];
       w[j] = mj == -INFINITY ? 0.f : fast_exp2(mj - m);
       l += w[j] * exchange_ml[2 * (j * kNarrowRows + at) + 1];
-      const floatx4 x = *reinterpret_cast<const floatx4 *>(
-          exchange + (j * kNarrowRows + at) * D + 4 * (piece ^ (at & 15)));
+      const floatx2 x = *reinterpret_cast<const floatx2 *>(
+          exchange + (j * kNarrowRows + at) * D + 4 * ((pair >> 1) ^ (at & 15)) + 2 * (pair & 1));
       if (mj != -INFINITY) o += w[j] * x;
     }
     if (it.slot < 0) {
       const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
-      o *= inv;
-      store4<T>(out_row<T>(p, it.t0, it.kvh, at, D) + 4 * piece, o);
+      typedef T t2 __attribute__((ext_vector_type(2)));
+      const t2 y = {static_cast<T>(o[0] * inv), static_cast<T>(o[1] * inv)};
+      *reinterpret_cast<t2 *>(out_row<T>(p, it.t0, it.kvh, at, D) + 2 * pair) = y;
     } else {
       float *part = partial_of(p, it.slot, D);
-      *reinterpret_cast<floatx4 *>(part + at * D + 4 * piece) = o;
-      if (piece == 0) {
-        part[p.slot_rows * D + 2 * at] = m;
-        part[p.slot_rows * D + 2 * at + 1] = l;
-      }
+      publish2(part + at * D + 2 * pair, o[0], o[1]);
+      if (pair == 0) publish2(part + p.slot_rows * D + 2 * at, m, l);
     }
   }
   block_barrier();  // the exchange may be overwritten
+}
+
+// Joins a narrow item's pieces, first to last, and writes its rows. Eight pieces' loads are
+// in flight at a time.
+template <typename T, int D>
+__device__ __forceinline__ void join_narrow(const AttendPagedParams &p, const Item &it,
+                                            const Pieces &pc) {
+  constexpr int kDeep = 8;
+  typedef T t2 __attribute__((ext_vector_type(2)));
+  const int n = it.n * p.group * (D / 2);
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const int row = i / (D / 2), at = 2 * (i % (D / 2));
+    float m = -INFINITY, l = 0.f;
+    floatx2 o = {0.f, 0.f};
+    for (int j0 = 0; j0 < pc.count; j0 += kDeep) {
+      floatx2 ml[kDeep], x[kDeep];
+#pragma unroll
+      for (int j = 0; j < kDeep; ++j) {
+        const int piece = min(j0 + j, pc.count - 1);
+        const int share = pc.first + piece - 1;
+        const float *part = partial_of(p, 2 * share + (piece == 0 ? 1 : 0), D);
+        ml[j] = fetch2(part + p.slot_rows * D + 2 * row);
+        x[j] = fetch2(part + row * D + at);
+      }
+#pragma unroll
+      for (int j = 0; j < kDeep; ++j) {
+        if (j0 + j >= pc.count || ml[j][0] == -INFINITY) continue;
+        const float top = fmaxf(m, ml[j][0]);
+        const float a = m == -INFINITY ? 0.f : fast_exp2(m - top), b = fast_exp2(ml[j][0] - top);
+        m = top;
+        l = l * a + ml[j][1] * b;
+        o = o * a + x[j] * b;
+      }
+    }
+    const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
+    const t2 y = {static_cast<T>(o[0] * inv), static_cast<T>(o[1] * inv)};
+    *reinterpret_cast<t2 *>(out_row<T>(p, it.t0, it.kvh, row, D) + at) = y;
+  }
 }
 
 template <typename T, int D>
@@ -644,31 +756,18 @@ __global__ __launch_bounds__(kThreads, 2) void attend_paged_kernel(const AttendP
   __shared__ __align__(16) float ml_mem[2 * kWaves * kNarrowRows];
   __shared__ int64_t wave_weight[kWaves];
   __shared__ Border borders[2];
+  __shared__ int arrived;
 
-  Record *records = static_cast<Record *>(p.records);
   const int tid = static_cast<int>(threadIdx.x);
   const int n_blocks = static_cast<int>(gridDim.x);
-
-  // Outputs of packed rows that belong to no sequence are zero.
-  {
-    const int lo = min(max(p.cu_tokens[0], 0), p.tokens);
-    const int hi = min(max(p.cu_tokens[p.batch], 0), p.tokens);
-    const int64_t per_row = static_cast<int64_t>(p.heads) * (D / 8);
-    const int64_t outside = (static_cast<int64_t>(lo) + p.tokens - hi) * per_row;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + tid; i < outside;
-         i += static_cast<int64_t>(n_blocks) * kThreads) {
-      const int64_t at = i < lo * per_row ? i : i + (static_cast<int64_t>(hi) - lo) * per_row;
-      const uint4 zero = {0, 0, 0, 0};
-      static_cast<uint4 *>(p.out)[at] = zero;
-    }
-  }
 
   // Every block sums the sequences' weights and finds its share's two borders.
   const int per = (p.batch + kThreads - 1) / kThreads;
   const int b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
   int64_t mine = 0;
+  Seq s = {0, 0, 0};
   for (int b = b0; b < b1; ++b) {
-    const Seq s = load_seq(p, b);
+    s = load_seq(p, b);
     const Tiles t = tiles_of(p, s.n);
     mine += weight_before(p, s, t, t.count) * p.kv_heads;
   }
@@ -679,7 +778,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend_paged_kernel(const AttendP
     if ((tid & 63) >= d) before += x;
   }
   if ((tid & 63) == 63) wave_weight[tid >> 6] = before;
-  if (tid < 2) borders[tid] = Border{p.batch, 0, 0, 0};
+  if (tid < 2) borders[tid].b = p.batch;
   __syncthreads();
   int64_t total = 0;
 #pragma unroll
@@ -688,12 +787,11 @@ __global__ __launch_bounds__(kThreads, 2) void attend_paged_kernel(const AttendP
     total += wave_weight[w];
   }
   before -= mine;
-  const int64_t share =
-      max((total + n_blocks - 1) / n_blocks, static_cast<int64_t>(kMinShareKeys));
-  const int active = static_cast<int>((total + share - 1) / share);
+  const int64_t share = max(floor_div(total, n_blocks) + 1, static_cast<int64_t>(kMinShareKeys));
   // Neighbouring shares read the same keys, so they go to one XCD (blocks are
   // dealt to the 8 XCDs in turn).
-  const int per_xcd = (active + 7) / 8;
+  const int active = static_cast<int>(floor_div(total, share)) + 1;
+  const int per_xcd = (min(active, n_blocks) + 7) / 8;
   const int blk = static_cast<int>(blockIdx.x);
   const int w = blk < 8 * per_xcd ? (blk & 7) * per_xcd + (blk >> 3) : blk;
 #pragma unroll 1
@@ -702,76 +800,61 @@ __global__ __launch_bounds__(kThreads, 2) void attend_paged_kernel(const AttendP
     if (at < before || at >= before + mine) continue;
     int64_t from = before;
     for (int b = b0; b < b1; ++b) {
-      const Seq s = load_seq(p, b);
+      if (per > 1) s = load_seq(p, b);
       const Tiles t = tiles_of(p, s.n);
       const int64_t whole = weight_before(p, s, t, t.count);
       if (at < from + whole * p.kv_heads) {
-        borders[side] = border_in(p, s, t, b, whole, at - from);
+        borders[side] = border_in(p, s, t, b, whole, from, at);
         break;
       }
       from += whole * p.kv_heads;
     }
   }
   __syncthreads();
-  Border cur = borders[0], end = borders[1];
-  cur.b = __builtin_amdgcn_readfirstlane(cur.b);
-  cur.kvh = __builtin_amdgcn_readfirstlane(cur.kvh);
-  cur.tile = __builtin_amdgcn_readfirstlane(cur.tile);
-  cur.kt = __builtin_amdgcn_readfirstlane(cur.kt);
-  end.b = __builtin_amdgcn_readfirstlane(end.b);
-  end.kvh = __builtin_amdgcn_readfirstlane(end.kvh);
-  end.tile = __builtin_amdgcn_readfirstlane(end.tile);
-  end.kt = __builtin_amdgcn_readfirstlane(end.kt);
+  auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  int b = uniform(borders[0].b), kvh = uniform(borders[0].kvh), tile = uniform(borders[0].tile);
+  int kt = uniform(borders[0].kt);
+  s.t0 = uniform(borders[0].s.t0);
+  s.n = uniform(borders[0].s.n);
+  s.p0 = uniform(borders[0].s.p0);
+  int64_t from = borders[0].from;
+  const int end_b = uniform(borders[1].b), end_kvh = uniform(borders[1].kvh);
+  const int end_tile = uniform(borders[1].tile), end_kt = uniform(borders[1].kt);
 
   const unsigned ring = lds_addr(ring_mem);
-  bool first = true;
-  Seq s = {0, 0, 0};
-  Tiles t = {0, 1};
-  int loaded = -1;
-  for (;;) {
-    if (cur.b >= p.batch) break;
-    if (loaded != cur.b) {
-      s = load_seq(p, cur.b);
-      s.t0 = __builtin_amdgcn_readfirstlane(s.t0);
-      s.n = __builtin_amdgcn_readfirstlane(s.n);
-      s.p0 = __builtin_amdgcn_readfirstlane(s.p0);
-      t = tiles_of(p, s.n);
-      loaded = cur.b;
-    }
-    if (cur.tile >= t.count) {  // next K/V head or sequence
-      cur.tile = 0;
-      cur.kt = 0;
-      if (t.count == 0 || ++cur.kvh >= p.kv_heads) {
-        cur.kvh = 0;
-        ++cur.b;
+  Tiles t = tiles_of(p, s.n);
+  while (b < p.batch) {
+    if (tile >= t.count) {  // next K/V head or sequence
+      tile = 0;
+      kt = 0;
+      if (t.count == 0 || ++kvh >= p.kv_heads) {
+        from += weight_before(p, s, t, t.count) * p.kv_heads;
+        kvh = 0;
+        ++b;
+        if (b >= p.batch) break;
+        s = load_seq(p, b);
+        s.t0 = uniform(s.t0);
+        s.n = uniform(s.n);
+        s.p0 = uniform(s.p0);
+        t = tiles_of(p, s.n);
       }
-      if (cur.b > end.b) break;
+      if (b > end_b) break;
       continue;
     }
-    const bool last = same_item(cur, end);
+    const bool last = b == end_b && kvh == end_kvh && tile == end_tile;
     Item it;
-    it.end = key_end(p, s, t, cur.tile);
-    const int tiles = (it.end + kTileKeys - 1) / kTileKeys;
-    it.kt0 = cur.kt;
-    it.kt1 = last ? min(end.kt, tiles) : tiles;
-    it.t0 = s.t0 + cur.tile * t.tokens;
-    it.n = min(t.tokens, s.n - cur.tile * t.tokens);
-    it.p0 = s.p0 + cur.tile * t.tokens;
-    it.kvh = cur.kvh;
+    it.end = key_end(p, s, t, tile);
+    const int tiles = key_tiles(it.end);
+    it.kt0 = kt;
+    it.kt1 = last ? min(end_kt, tiles) : tiles;
+    it.t0 = s.t0 + tile * t.tokens;
+    it.n = min(t.tokens, s.n - tile * t.tokens);
+    it.p0 = s.p0 + tile * t.tokens;
+    it.kvh = kvh;
     it.table = (uniform_table)(reinterpret_cast<uintptr_t>(
-        p.page_table + static_cast<int64_t>(cur.b) * p.max_pages));
-    if (first && tid == 0) {
-      Record rec;
-      rec.at = cur;
-      rec.tiles = tiles;
-      rec.t0 = it.t0;
-      rec.n = it.n;
-      rec.pad = 0;
-      records[w] = rec;
-    }
-    first = false;
+        p.page_table + static_cast<int64_t>(b) * p.max_pages));
     // A whole item (also one that sees no key) is written out; a part leaves a partial.
-    const bool whole = it.kt0 == 0 && it.kt1 == tiles && !(last && end.kt < tiles) &&
+    const bool whole = it.kt0 == 0 && it.kt1 == tiles && !(last && end_kt < tiles) &&
                        !(last && tiles == 0);
     if (whole || it.kt1 > it.kt0) {
       it.slot = whole ? -1 : 2 * w + (it.kt0 == 0 ? 1 : 0);
@@ -780,67 +863,51 @@ __global__ __launch_bounds__(kThreads, 2) void attend_paged_kernel(const AttendP
       else
         wide_item<T, D>(p, it, ring);
     }
+    if (!whole && it.kt1 > it.kt0) {
+      const int64_t x0 = from + kvh * weight_before(p, s, t, t.count) + weight_before(p, s, t, tile);
+      const int64_t x1 = x0 + weight_before(p, s, t, tile + 1) - weight_before(p, s, t, tile);
+      const Pieces pc = pieces_of(x0, x1, tiles, share);
+      // The partial is stored before it is counted; the block that counts last sets the
+      // counter back to zero for the next call.
+      wait_loads<0>();
+      __syncthreads();
+      if (tid == 0) {
+        unsigned *counter = p.counters + pc.first;
+        const unsigned n = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED,
+                                                  __HIP_MEMORY_SCOPE_AGENT);
+        arrived = static_cast<int>(n) + 1;
+        if (arrived == pc.count)
+          __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+      __syncthreads();
+      if (arrived == pc.count) {
+        if (it.n * p.group <= kNarrowRows) join_narrow<T, D>(p, it, pc);
+        else join_wide<T, D>(p, it, pc);
+      }
+      __syncthreads();
+    }
     if (last) break;
-    ++cur.tile;
-    cur.kt = 0;
+    ++tile;
+    kt = 0;
   }
-  if (first && tid == 0) {
-    Record rec;
-    rec.at = Border{-1, 0, 0, 0};
-    rec.tiles = rec.t0 = rec.n = rec.pad = 0;
-    records[w] = rec;
+
+  // Outputs of packed rows that belong to no sequence are zero.
+  const int lo = min(max(p.cu_tokens[0], 0), p.tokens);
+  const int hi = min(max(p.cu_tokens[p.batch], 0), p.tokens);
+  const int64_t per_row = static_cast<int64_t>(p.heads) * (D / 8);
+  const int64_t outside = (static_cast<int64_t>(lo) + p.tokens - hi) * per_row;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + tid; i < outside;
+       i += static_cast<int64_t>(n_blocks) * kThreads) {
+    const int64_t at = i < lo * per_row ? i : i + (static_cast<int64_t>(hi) - lo) * per_row;
+    const uint4 zero = {0, 0, 0, 0};
+    static_cast<uint4 *>(p.out)[at] = zero;
   }
 }
 
-// Joins the partials of an item that borders cut: block (w, y) takes rows
-// [8 y, +8) of the item whose first inner border is share w's.
-template <typename T, int D>
-__global__ __launch_bounds__(kThreads) void attend_merge_kernel(const AttendPagedParams p,
-                                                                int n_blocks) {
-  const Record *records = static_cast<const Record *>(p.records);
-  const int w = static_cast<int>(blockIdx.x) + 1;
-  const Record rec = records[w];
-  if (rec.at.b < 0 || rec.at.kt <= 0) return;
-  const Record prev = records[w - 1];
-  if (same_item(prev.at, rec.at) && prev.at.kt > 0) return;
-  if (rec.at.kt >= rec.tiles) return;  // the share before holds the whole item
-  const int wave = static_cast<int>(threadIdx.x) >> 6, lane = static_cast<int>(threadIdx.x) & 63;
-  constexpr int kPer = D / 64;  // dims per lane
-  for (int row = kMergeRows * blockIdx.y + wave; row < kMergeRows * (static_cast<int>(blockIdx.y) + 1);
-       row += kWaves) {
-    if (row >= rec.n * p.group) return;
-    float m = -INFINITY, l = 0.f, o[kPer] = {};
-    auto add = [&](int slot) {
-      const float *part = partial_of(p, slot, D);
-      const float pm = part[p.slot_rows * D + 2 * row];
-      const float pl = part[p.slot_rows * D + 2 * row + 1];
-      float x[kPer];
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) x[i] = part[row * D + kPer * lane + i];
-      if (pm == -INFINITY) return;
-      const float top = fmaxf(m, pm);
-      const float a = m == -INFINITY ? 0.f : fast_exp2(m - top), b = fast_exp2(pm - top);
-      m = top;
-      l = l * a + pl * b;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) o[i] = o[i] * a + x[i] * b;
-    };
-    add(2 * (w - 1) + 1);
-    int kt = rec.at.kt;
-    for (int j = w; j < n_blocks && kt < rec.tiles; ++j) {
-      int next = rec.tiles;
-      if (j + 1 < n_blocks) {
-        const Record r = records[j + 1];
-        if (r.at.b >= 0 && same_item(r.at, rec.at)) next = r.at.kt;
-      }
-      if (next > kt) add(2 * j);
-      kt = next;
-    }
-    const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
-    T *out = out_row<T>(p, rec.t0, rec.at.kvh, row, D) + kPer * lane;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) out[i] = static_cast<T>(o[i] * inv);
-  }
+// Zeroes the arrival counters of a call whose stream has no counter slot.
+__global__ void zero_counters_kernel(unsigned *counters, int n) {
+  const int i = static_cast<int>(blockIdx.x * blockDim.x + threadIdx.x);
+  if (i < n) counters[i] = 0;
 }
 
 int attend_blocks() {
@@ -849,27 +916,23 @@ int attend_blocks() {
   return 2 * device_cu_count(dev);
 }
 int slot_rows_of(int tokens, int group) {
-  return static_cast<int>(
-      min(static_cast<int64_t>(kWideRows), static_cast<int64_t>(tokens) * group));
+  return static_cast<int64_t>(tokens) * group <= kNarrowRows ? kNarrowRows : kWideRows;
 }
 
 template <typename T, int D>
 int launch(const AttendPagedParams &p, int n_blocks, hipStream_t stream) {
   hipLaunchKernelGGL((attend_paged_kernel<T, D>), dim3(static_cast<unsigned>(n_blocks)),
                      dim3(kThreads), 0, stream, p);
-  int rc = check_hip(hipGetLastError(), "attend_paged_kernel launch");
-  if (rc != FA_OK) return rc;
-  const unsigned groups = static_cast<unsigned>((p.slot_rows + kMergeRows - 1) / kMergeRows);
-  hipLaunchKernelGGL((attend_merge_kernel<T, D>), dim3(static_cast<unsigned>(n_blocks - 1), groups),
-                     dim3(kThreads), 0, stream, p, n_blocks);
-  return check_hip(hipGetLastError(), "attend_merge_kernel launch");
+  return check_hip(hipGetLastError(), "attend_paged_kernel launch");
 }
+
+size_t counter_bytes(size_t n) { return (n * sizeof(unsigned) + 255) / 256 * 256; }
 
 }  // namespace
 
 size_t attend_paged_workspace_bytes(int tokens, int group, int head_dim) {
   const size_t n = static_cast<size_t>(attend_blocks());
-  return n * sizeof(Record) +
+  return counter_bytes(n) +
          2 * n * slot_rows_of(tokens, group) * (static_cast<size_t>(head_dim) + 2) * sizeof(float);
 }
 
@@ -884,9 +947,18 @@ int launch_attend_paged(AttendPagedParams p, bool bf16, int head_dim, float scal
   // zero one becomes the least that keeps a hidden key's -inf (-inf * 0 is NaN).
   p.negate = scale < 0.f;
   p.c = fmaxf(fabsf(scale) * kLog2e, 1e-37f);
-  p.records = workspace;
   p.partials = reinterpret_cast<float *>(static_cast<char *>(workspace) +
-                                         static_cast<size_t>(n_blocks) * sizeof(Record));
+                                         counter_bytes(static_cast<size_t>(n_blocks)));
+  // Arrival counters: the stream's own, zero between calls, or, where it has no slot,
+  // the workspace's, zeroed by a launch of their own.
+  p.counters = merge_counters(stream, static_cast<size_t>(n_blocks));
+  if (p.counters == nullptr) {
+    p.counters = static_cast<unsigned *>(workspace);
+    hipLaunchKernelGGL(zero_counters_kernel, dim3(static_cast<unsigned>((n_blocks + 255) / 256)),
+                       dim3(256), 0, stream, p.counters, n_blocks);
+    const int rc = check_hip(hipGetLastError(), "zero_counters_kernel launch");
+    if (rc != FA_OK) return rc;
+  }
   if (head_dim == 64)
     return bf16 ? launch<__bf16, 64>(p, n_blocks, stream) : launch<_Float16, 64>(p, n_blocks, stream);
   return bf16 ? launch<__bf16, 128>(p, n_blocks, stream) : launch<_Float16, 128>(p, n_blocks, stream);
