@@ -160,7 +160,8 @@ def m0_problems(asm: str) -> list:
     """Every instruction in `asm` (AMDGPU assembly) that defines or reads m0
     other than the global_to_lds16 pattern `s_mov_b32 m0, <SGPR>` [s_nop ...]
     `global_load_lds_dwordx4`, and every global_load_lds without that write
-    right before it."""
+    right before it. A load with an `offset:` may also follow another load: it
+    continues that one's m0 (load_slab in csrc/paged.hip)."""
     code = []
     for raw in asm.splitlines():
         ins = raw.split(";", 1)[0].strip()
@@ -173,6 +174,8 @@ def m0_problems(asm: str) -> list:
             j = i - 1
             while j >= 0 and code[j].startswith("s_nop"):
                 j -= 1
+            if "offset:" in ins and j >= 0 and code[j].startswith("global_load_lds"):
+                continue
             if j < 0 or not _M0_WRITE.match(code[j]):
                 problems.append(f"global_load_lds without its m0 write: {ins}")
         elif re.search(r"\bm0\b", ins):

@@ -687,15 +687,6 @@ struct GroupGeo {
   static constexpr int kWavesPerCu = (160 * 1024) / (2 * kStages * kTileHalves * 2);
 };
 
-// V chunk swizzle of the grouped tiles (a 32-lane transpose-read phase reads
-// the chunk pair {2 d, 2 d + 1} of 8 consecutive rows): 8 distinct 32-byte
-// places in the 256 bytes that two 128-byte rows, or one 256-byte row, span.
-template <int D>
-__device__ __forceinline__ int group_v_swz(int row) {
-  if constexpr (D == 64) return ((row >> 1) & 3) << 1;
-  else return (row & 7) << 1;
-}
-
 // Wait until a ring tile is resident while the `later` (<= K) tiles issued
 // after it, L loads each, may still fly (vmcnt counts at most 63).
 template <int K, int L>
@@ -709,20 +700,6 @@ __device__ __forceinline__ void wait_ring(int later) {
     else
       wait_ring<K - 1, L>(later);
   }
-}
-
-// max(x[l], x[l ^ 16], x[l ^ 32], x[l ^ 48]) for every lane (VALU only, no
-// LDS). As in max_lane_pair the swaps are written in asm: the compiler treats
-// a swap of two equal values as a no-op.
-__device__ __forceinline__ float max_lane_groups(float x) {
-  float a = max_lane_pair(x), b = a;
-  asm volatile(
-      "s_nop 1\n\t"
-      "v_permlane16_swap_b32 %0, %1\n\t"
-      "s_nop 0\n\t"
-      "v_max_f32 %0, %0, %1"
-      : "+v"(a), "+v"(b));
-  return a;
 }
 
 template <int D, int QB>

@@ -121,6 +121,9 @@ struct AttendPagedParams {
   int batch, tokens, heads, kv_heads, num_pages, page_shift, max_pages;
   // Set by the launcher.
   int group, slot_rows, capacity;
+  int wide_tokens, narrow_tokens, narrow_step, group_inv, unit, min_share;
+  unsigned blocks_inv, head_bytes, page_bytes;
+  float wide_inv;
   float c;
   bool negate;
   unsigned *counters;

@@ -241,6 +241,28 @@ __device__ __forceinline__ float max_lane_pair(float x) {
   return a;
 }
 
+// max(x[l], x[l ^ 16], x[l ^ 32], x[l ^ 48]) for every lane (VALU only, no
+// LDS). As in max_lane_pair the swaps are written in asm: the compiler treats
+// a swap of two equal values as a no-op.
+__device__ __forceinline__ float max_lane_groups(float x) {
+  float a = max_lane_pair(x), b = a;
+  asm volatile(
+      "s_nop 1\n\t"
+      "v_permlane16_swap_b32 %0, %1\n\t"
+      "s_nop 0\n\t"
+      "v_max_f32 %0, %0, %1"
+      : "+v"(a), "+v"(b));
+  return a;
+}
+
+// V chunk swizzle of the grouped tiles (a 32-lane transpose-read phase reads
+// the chunk pair {2 d, 2 d + 1} of 8 consecutive rows): 8 distinct 32-byte
+// places in the 256 bytes that two 128-byte rows, or one 256-byte row, span.
+template <int D>
+__device__ __forceinline__ int group_v_swz(int row) {
+  if constexpr (D == 64) return ((row >> 1) & 3) << 1;
+  else return (row & 7) << 1;
+}
 
 // Partials that another wave of the same launch reads: relaxed agent-scope
 // atomic stores and loads, which go to the device-coherent level (sc1) on

@@ -28,8 +28,8 @@
 //     tiles in an LDS ring filled by direct global->LDS loads.
 //   narrow item: the waves take key tiles in turn, each with K and V tiles of its
 //     own in LDS (no barrier in the loop), and join their states at the end.
-//   Products on v_mfma_f32_32x32x16: S^T = K Q^T, O^T += V^T P^T (mfma_tile.h), a
-//   query row per lane pair.
+//   Products on v_mfma_f32_32x32x16 (wide; mfma_tile.h) and 16x16x32 (narrow): S^T = K Q^T,
+//   O^T += V^T P^T, so a query row's scores lie in one lane pair, or four lanes.
 //
 // Roundings to 16 bits. P is rounded once on wide items (the row sum is taken of
 // the rounded weights, so a row that one key carries is exact) and split into two
@@ -95,17 +95,23 @@ __device__ __forceinline__ frag_t<T> ones_selector(int lane) {
 
 // ---- sequences, items and shares ------------------------------------------------
 
+typedef const __attribute__((address_space(4))) int32_t *uniform_ints;  // read with scalar loads
+__device__ __forceinline__ uniform_ints uniform_at(const int32_t *p) {
+  return (uniform_ints)(reinterpret_cast<uintptr_t>(p));
+}
+
 // A sequence's new tokens: packed rows [t0, t0 + n), the first at position p0.
 struct Seq {
   int t0, n, p0;
 };
-__device__ __forceinline__ Seq load_seq(const AttendPagedParams &p, int b) {
-  const int lo = p.cu_tokens[b], hi = p.cu_tokens[b + 1];
+template <typename Ints>
+__device__ __forceinline__ Seq load_seq(const AttendPagedParams &p, Ints bounds, Ints lens, int b) {
+  const int lo = bounds[b], hi = bounds[b + 1];
   Seq s;
   s.t0 = min(max(lo, 0), p.tokens);
   s.n = min(max(hi, s.t0), p.tokens) - s.t0;
-  // seq_lens - hi + t0, kept far from overflow whatever the buffers hold.
-  const int64_t p0 = static_cast<int64_t>(p.seq_lens[b]) - hi + s.t0;
+  // lens[b] - hi + t0, kept far from overflow whatever the buffers hold.
+  const int64_t p0 = static_cast<int64_t>(lens[b]) - hi + s.t0;
   s.p0 = static_cast<int>(min(max(p0, static_cast<int64_t>(-(1 << 30))),
                               static_cast<int64_t>(1 << 30)));
   return s;
@@ -113,91 +119,121 @@ __device__ __forceinline__ Seq load_seq(const AttendPagedParams &p, int b) {
 // Items of a sequence (per K/V head): `count` tiles of `tokens` tokens.
 struct Tiles {
   int count, tokens;
+  int step;  // borders inside its items lie at multiples of this many key tiles
 };
+template <bool SCALAR>  // n is the wave's, not the lane's
 __device__ __forceinline__ Tiles tiles_of(const AttendPagedParams &p, int n) {
   Tiles t;
-  const bool narrow = n <= kNarrowRows / p.group;
-  t.tokens = narrow ? max(n, 1) : kWideRows / p.group;
-  t.count = narrow ? (n > 0 ? 1 : 0) : (n + t.tokens - 1) / t.tokens;
+  const bool narrow = n <= p.narrow_tokens;
+  t.tokens = narrow ? max(n, 1) : p.wide_tokens;
+  t.step = narrow ? p.narrow_step : 1;
+  // n / wide_tokens, rounded up, by its reciprocal (n < 2^24: exact in fp32 to within one).
+  int q = static_cast<int>(static_cast<float>(n) * p.wide_inv);
+  q += q * p.wide_tokens < n;
+  q -= (q - 1) * p.wide_tokens >= n;
+  if constexpr (SCALAR) q = __builtin_amdgcn_readfirstlane(q);
+  t.count = narrow ? (n > 0 ? 1 : 0) : q;
   return t;
 }
 // Keys the last token of a tile sees.
 __device__ __forceinline__ int key_end(const AttendPagedParams &p, const Seq &s, const Tiles &t,
                                        int tile) {
-  const int64_t last = static_cast<int64_t>(s.p0) +
-                       min(static_cast<int64_t>(s.n), static_cast<int64_t>(tile + 1) * t.tokens);
-  return static_cast<int>(min(max(last, int64_t{0}), static_cast<int64_t>(p.capacity)));
+  // p0 + n <= 2^30 + 2^24
+  return min(max(s.p0 + min(s.n, (tile + 1) * t.tokens), 0), p.capacity);
 }
 // Weight of tiles [0, tile) of one K/V head: the keys each tile sees (taken as
-// if the last tile were whole) plus a fixed cost per item.
-__device__ __forceinline__ int64_t weight_before(const AttendPagedParams &p, const Seq &s,
-                                                 const Tiles &t, int tile) {
-  const int64_t each = static_cast<int64_t>(min(max(s.p0, 0), p.capacity)) + kItemKeys;
-  return tile * each + static_cast<int64_t>(t.tokens) * tile * (tile + 1) / 2;
+// if the last tile were whole) plus a fixed cost per item, in units of 2^unit
+// keys, at least one per item. The host picks the unit that keeps a batch's
+// weight within 30 bits (one key, but for batches of 10^9 keys and more).
+__device__ __forceinline__ int weight_before(const AttendPagedParams &p, const Seq &s,
+                                             const Tiles &t, int tile) {
+  const int each = min(max(s.p0, 0), p.capacity) + kItemKeys;
+  const int64_t keys = static_cast<int64_t>(tile) * each +
+                       (static_cast<int64_t>(tile) * (tile + 1) >> 1) * t.tokens;
+  return tile + static_cast<int>(keys >> p.unit);
 }
 
 // Key tiles of an item.
 __device__ __forceinline__ int key_tiles(int end) { return (end + kTileKeys - 1) / kTileKeys; }
 
-// floor(a / b) for 0 <= a < 2^52, b > 0: a product in fp64 (one estimate off by at
-// most one, then corrected) instead of a 64-bit integer division, which costs
-// over a hundred dependent instructions at the start of every block.
-__device__ __forceinline__ int64_t floor_div(int64_t a, int64_t b) {
-  int64_t q = static_cast<int64_t>(static_cast<double>(a) / static_cast<double>(b));
-  if (q * b > a) --q;
-  if ((q + 1) * b <= a) ++q;
-  return q;
+// a / b for 0 <= a < 2^31, 0 < b, quotients below 2^20: a product in fp32, off by at
+// most one, corrected. (64-bit integer divisions took 2 us at the start of every block.)
+__device__ __forceinline__ int floor_div(int a, int b) {
+  int q = static_cast<int>(static_cast<float>(a) * __builtin_amdgcn_rcpf(static_cast<float>(b)));
+  const int64_t r = a - static_cast<int64_t>(q) * b;
+  return q + (r >= b ? 1 : r < 0 ? -1 : 0);
 }
-__device__ __forceinline__ int64_t ceil_div(int64_t a, int64_t b) { return floor_div(a + b - 1, b); }
 
 // A share's border: before key tile `kt` of item (b, kvh, tile); `from` is the weight
 // of the sequences before b.
 struct Border {
   int b, kvh, tile, kt;
   Seq s;
-  int pad;
-  int64_t from;
+  int from;
 };
 
 // The border at weight `at` inside sequence b (0 <= at - from < H_kv * whole).
-__device__ Border border_in(const AttendPagedParams &p, const Seq &s, const Tiles &t, int b,
-                            int64_t whole, int64_t from, int64_t at) {
-  Border r;
-  r.b = b;
-  r.s = s;
-  r.from = from;
-  at -= from;
-  r.kvh = static_cast<int>(floor_div(at, whole));
+__device__ __forceinline__ void place_border(const AttendPagedParams &p, const Tiles &t, int at,
+                                             Border &r) {
+  const int whole = weight_before(p, r.s, t, t.count);
+  at -= r.from;
+  r.kvh = floor_div(at, whole);
   at -= r.kvh * whole;
   int lo = 0, hi = t.count;  // the last tile whose weight_before is <= at
   while (hi - lo > 1) {
     const int mid = (lo + hi) / 2;
-    if (weight_before(p, s, t, mid) <= at) lo = mid;
+    if (weight_before(p, r.s, t, mid) <= at) lo = mid;
     else hi = mid;
   }
   r.tile = lo;
-  const int tiles = key_tiles(key_end(p, s, t, lo));
-  const int64_t in = at - weight_before(p, s, t, lo) - kItemKeys;
+  const int tiles = key_tiles(key_end(p, r.s, t, lo));
+  const int64_t in =
+      (static_cast<int64_t>(at - weight_before(p, r.s, t, lo)) << p.unit) - kItemKeys;
   r.kt = static_cast<int>(min(max(in, int64_t{0}) / kTileKeys, static_cast<int64_t>(tiles)));
   // A border close to an item's end moves there: a partial costs more than the keys it balances.
-  if (r.kt < kSnapTiles) r.kt = 0;
-  else if (r.kt > tiles - kSnapTiles) r.kt = tiles;
-  return r;
+  r.kt -= r.kt % t.step;
+  if (r.kt > tiles - kSnapTiles) r.kt = tiles;
 }
 
 // The shares that an item of `tiles` key tiles at weights [x0, x1) is cut into: the
 // first border inside it and the number of pieces. Piece i is share
-// first + i - 1's; a border k lies inside when border_in gives it 0 < kt < tiles.
+// first + i - 1's; a border k lies inside when place_border gives it 0 < kt < tiles.
 struct Pieces {
   int first, count;
 };
-__device__ __forceinline__ Pieces pieces_of(int64_t x0, int64_t x1, int tiles, int64_t share) {
+__device__ __forceinline__ int ceil_units(const AttendPagedParams &p, int64_t keys) {
+  return static_cast<int>((keys + (int64_t{1} << p.unit) - 1) >> p.unit);
+}
+__device__ __forceinline__ Pieces pieces_of(const AttendPagedParams &p, const Tiles &t, int x0,
+                                            int x1, int tiles, int share) {
   Pieces r;
-  r.first = static_cast<int>(ceil_div(x0 + kItemKeys + kSnapTiles * kTileKeys, share));
-  const int64_t stop =
-      min(x1, x0 + kItemKeys + static_cast<int64_t>(tiles - kSnapTiles + 1) * kTileKeys);
-  r.count = static_cast<int>(ceil_div(stop, share)) - r.first + 1;
+  const int start = x0 + ceil_units(p, kItemKeys + t.step * kTileKeys);
+  r.first = __builtin_amdgcn_readfirstlane(floor_div(start + share - 1, share));
+  const int64_t beyond = tiles - kSnapTiles - (tiles - kSnapTiles) % t.step + t.step;
+  const int stop = min(x1, x0 + ceil_units(p, kItemKeys + beyond * kTileKeys));
+  r.count = __builtin_amdgcn_readfirstlane(floor_div(stop + share - 1, share)) - r.first + 1;
   return r;
+}
+
+// Inclusive sum over the wave's lanes (DPP row shifts and broadcasts).
+__device__ __forceinline__ int wave_prefix(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);   // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);   // row_shr:2
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);   // row_shr:4
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);   // row_shr:8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast:15, rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast:31, rows 2 and 3
+  return x;
+}
+
+// A V^T operand from two transposed reads (four keys each) of a V tile.
+template <typename T>
+__device__ __forceinline__ frag_t<T> read_v(lds_half *first, lds_half *second) {
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) short4v lds_short4;
+  const t4 a = __builtin_bit_cast(t4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)first));
+  const t4 b = __builtin_bit_cast(t4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)second));
+  return frag_t<T>{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
 
 // ---- a wave's rows -----------------------------------------------------------------
@@ -222,23 +258,38 @@ __device__ __forceinline__ void clear_rows(Rows<T, D> &r) {
   r.m = -INFINITY;
 }
 
-// Loads the lane's query row `row` of an item (rows past the last repeat it).
-template <typename T, int D>
-__device__ __forceinline__ void load_queries(const AttendPagedParams &p, int t0, int n, int p0,
-                                             int kvh, int row, int g, Rows<T, D> &r) {
-  row = min(row, n * p.group - 1);
-  const int token = row / p.group;
-  const int head = kvh * p.group + row - token * p.group;
-  const T *q = static_cast<const T *>(p.q) + static_cast<int64_t>(t0 + token) * p.q_token +
-               static_cast<int64_t>(head) * p.q_head;
-  r.pos = p0 + token;
+// row / group for row < 128, by the host's ceil(2^16 / group): exact, the product is over
+// by less than 128 / 2^16 < 1 / group.
+__device__ __forceinline__ int token_of(const AttendPagedParams &p, int row) {
+  return (row * p.group_inv) >> 16;
+}
+
+struct Item {
+  int t0, n, p0;     // packed tokens and the first one's position
+  int kvh;
+  int kt0, kt1;      // key tiles of this share
+  int end;           // keys the item sees (the last token's)
+  int slot;          // partial slot, -1: the whole item
+  uniform_ints table;
+  const char *k, *v;  // the K/V head's rows of page 0
+};
+
+// An item's query row, and its position.
+template <typename T>
+__device__ __forceinline__ const T *query_row(const AttendPagedParams &p, const Item &it, int row,
+                                              int &pos) {
+  const int token = token_of(p, row);
+  const int head = it.kvh * p.group + row - token * p.group;
+  pos = it.p0 + token;
+  return static_cast<const T *>(p.q) + static_cast<int64_t>(it.t0 + token) * p.q_token +
+         static_cast<int64_t>(head) * p.q_head;
+}
+template <typename T>
+__device__ __forceinline__ frag_t<T> load_query(const AttendPagedParams &p, const T *q) {
   const unsigned flip = p.negate ? 0x80008000u : 0u;  // a negative scale: -q, exactly
-#pragma unroll
-  for (int s = 0; s < D / 16; ++s) {
-    uint4 x = *reinterpret_cast<const uint4 *>(q + (D / 2) * g + 8 * s);
-    x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
-    r.q[s] = __builtin_bit_cast(frag_t<T>, x);
-  }
+  uint4 x = *reinterpret_cast<const uint4 *>(q);
+  x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
+  return __builtin_bit_cast(frag_t<T>, x);
 }
 
 // ---- one tile of KB 32-key blocks: scores, softmax, products ------------------------
@@ -278,12 +329,12 @@ __device__ __forceinline__ void hide(floatx16 (&s)[KB], int lim, unsigned absent
     }
 }
 
-// Weights of the tile as P^T fragments (SPLIT: lo holds what hi lost). The bound m
+// Weights of the tile as P^T fragments. The bound m
 // moves only when a row's scores pass it by more than 2^8 (weights up to 2^8 are
 // harmless in either type): O is rescaled a few times per item instead of per tile.
-template <typename T, int D, int KB, bool SPLIT>
+template <typename T, int D, int KB>
 __device__ __forceinline__ void weigh(floatx16 (&s)[KB], float c, Rows<T, D> &r,
-                                      frag_t<T> (&hi)[2 * KB], frag_t<T> (&lo)[2 * KB]) {
+                                      frag_t<T> (&w)[2 * KB]) {
   float mx = -INFINITY;
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb)
@@ -304,98 +355,132 @@ __device__ __forceinline__ void weigh(floatx16 (&s)[KB], float c, Rows<T, D> &r,
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-    for (int a = 0; a < 16; ++a) {
-      const float w = fast_exp2(__builtin_fmaf(s[kb][a], c, -m));
-      const T h = static_cast<T>(w);
-      hi[2 * kb + (a >> 3)][a & 7] = h;
-      if constexpr (SPLIT) lo[2 * kb + (a >> 3)][a & 7] = static_cast<T>(w - static_cast<float>(h));
-    }
+    for (int a = 0; a < 16; ++a)
+      w[2 * kb + (a >> 3)][a & 7] = static_cast<T>(fast_exp2(__builtin_fmaf(s[kb][a], c, -m)));
 }
 
-template <typename T, int D, int KB, bool SPLIT>
+template <typename T, int D, int KB>
 __device__ __forceinline__ void accumulate(unsigned tile, const FragOffsetsD<D> &fo,
-                                           const frag_t<T> &ones, const frag_t<T> (&hi)[2 * KB],
-                                           const frag_t<T> (&lo)[2 * KB], Rows<T, D> &r) {
+                                           const frag_t<T> &ones, const frag_t<T> (&w)[2 * KB],
+                                           Rows<T, D> &r) {
   const unsigned base = uniform_lds_u(tile);
 #pragma unroll
-  for (int ks = 0; ks < 2 * KB; ++ks) {
-    r.l = Frag<T>::mm16(ones, hi[ks], r.l);
-    if constexpr (SPLIT) r.l = Frag<T>::mm16(ones, lo[ks], r.l);
-  }
+  for (int ks = 0; ks < 2 * KB; ++ks) r.l = Frag<T>::mm16(ones, w[ks], r.l);
 #pragma unroll
   for (int db = 0; db < D / 32; ++db) {
     lds_half *at = opaque_lds_at(base, fo.v[db]);
 #pragma unroll
-    for (int ks = 0; ks < 2 * KB; ++ks) {
-      frag_t<T> v;
-#pragma unroll
-      for (int part = 0; part < 2; ++part) {
-        const short4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) short4v *)(at + (ks * 16 + 8 * part) * D));
-        typedef T t4 __attribute__((ext_vector_type(4)));
-        const t4 y = __builtin_bit_cast(t4, x);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[4 * part + e] = y[e];
-      }
-      r.o[db] = Frag<T>::mm(v, hi[ks], r.o[db]);
-      if constexpr (SPLIT) r.o[db] = Frag<T>::mm(v, lo[ks], r.o[db]);
-    }
+    for (int ks = 0; ks < 2 * KB; ++ks)
+      r.o[db] = Frag<T>::mm(read_v<T>(at + ks * 16 * D, at + (ks * 16 + 8) * D), w[ks], r.o[db]);
   }
 }
 
 // ---- pages --------------------------------------------------------------------------
 
-typedef const __attribute__((address_space(4))) int32_t *uniform_table;
-
-// Where 16 consecutive keys of one K/V head begin; `absent` where their page id
-// is outside the pool (the address is page 0's then).
-struct Slab {
-  int64_t at;  // in rows of head_dim elements
-  bool absent;
+// Page ids of the N 16-key slabs from `key` on: N scalar loads, in flight together. Keys
+// past the end lie on no page of their own: the last key's page stands in.
+template <int N>
+struct PageIds {
+  int id[N];
 };
-__device__ __forceinline__ Slab slab_of(const AttendPagedParams &p, uniform_table table, int kvh,
-                                        int key, int end) {
-  // Keys past the end lie on no page of their own: the last key's page stands in.
-  if (key >= end) key = (end - 1) & ~15;
-  const int page = __builtin_amdgcn_readfirstlane(table[key >> p.page_shift]);
-  Slab s;
-  s.absent = static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_pages);
-  const int64_t id = s.absent ? 0 : page;
-  s.at = ((id * p.kv_heads + kvh) << p.page_shift) + (key & ((1 << p.page_shift) - 1));
-  return s;
+template <int N>
+__device__ __forceinline__ PageIds<N> page_ids(const AttendPagedParams &p, const Item &it,
+                                               int key) {
+  PageIds<N> r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) r.id[i] = it.table[min(key + 16 * i, it.end - 1) >> p.page_shift];
+  return r;
+}
+__device__ __forceinline__ bool is_absent(const AttendPagedParams &p, int id) {
+  return static_cast<unsigned>(id) >= static_cast<unsigned>(p.num_pages);
+}
+// Bit i: slab i lies on a page outside the pool.
+template <int N>
+__device__ __forceinline__ unsigned absent_of(const AttendPagedParams &p, const PageIds<N> &ids) {
+  unsigned absent = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) absent |= is_absent(p, ids.id[i]) ? 1u << i : 0u;
+  return absent;
+}
+// Byte offsets, from the K/V head's rows of page 0, of the 16 keys from `key` + 16 i on, which
+// lie in one page; page 0 stands in for one outside the pool. K and V share them.
+template <int N>
+struct Slabs {
+  uint64_t at[N];
+};
+template <int D, int N>
+__device__ __forceinline__ Slabs<N> slabs_of(const AttendPagedParams &p, const Item &it,
+                                             const PageIds<N> &ids, int key) {
+  Slabs<N> r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const unsigned page = is_absent(p, ids.id[i]) ? 0u : static_cast<unsigned>(ids.id[i]);
+    const unsigned row = static_cast<unsigned>(key + 16 * i) & ((1u << p.page_shift) - 1);
+    r.at[i] = static_cast<uint64_t>(page) * p.page_bytes + row * (D * 2);
+  }
+  return r;
 }
 
-// Per-lane source offsets (bytes) of the 16-byte pieces that fill 16 rows of a K
-// or V tile; a load instruction writes 1 KiB of LDS, 64 / (D / 8) rows.
-template <int D>
+// Per-lane source offsets (bytes) of the 16-byte pieces that fill 16 rows of a K or V
+// tile: load instruction j writes 1 KiB of LDS, 64 / (D / 8) rows, and adds 1024 j itself.
+template <int D, bool NARROW>
 struct LoadOffsets {
-  static constexpr int kLoads = D / 32;  // instructions per 16 rows
-  unsigned k[kLoads], v[kLoads];
+  unsigned k[D / 32], v[D / 32];
 };
-template <int D>
-__device__ __forceinline__ LoadOffsets<D> load_offsets(int lane) {
-  LoadOffsets<D> lo;
+template <int D, bool NARROW>
+__device__ __forceinline__ LoadOffsets<D, NARROW> load_offsets(int lane) {
+  LoadOffsets<D, NARROW> lo;
   constexpr int kChunks = D / 8;
+  const int chunk = lane % kChunks, row0 = lane / kChunks;
 #pragma unroll
-  for (int j = 0; j < LoadOffsets<D>::kLoads; ++j) {
-    const int row = j * (64 / kChunks) + lane / kChunks;
-    const int chunk = lane % kChunks;
-    lo.k[j] = static_cast<unsigned>(row * D + ((chunk ^ k_swz_d<D>(row)) << 3)) * 2;
-    lo.v[j] = static_cast<unsigned>(row * D + ((chunk ^ v_swz_d<D>(row)) << 3)) * 2;
+  for (int j = 0; j < D / 32; ++j) {
+    const int row = j * (64 / kChunks) + row0;
+    const int v_swz = NARROW ? group_v_swz<D>(row) : v_swz_d<D>(row);
+    lo.k[j] = static_cast<unsigned>(row0 * D + ((chunk ^ k_swz_d<D>(row)) << 3)) * 2;
+    lo.v[j] = static_cast<unsigned>(row0 * D + ((chunk ^ v_swz) << 3)) * 2;
   }
   return lo;
 }
-template <int D>
-__device__ __forceinline__ void load_slab(const void *pages, int64_t at,
-                                          const unsigned (&off)[LoadOffsets<D>::kLoads],
-                                          unsigned lds, bool once) {
-  const char *base = static_cast<const char *>(pages) + at * (D * 2);
-#pragma unroll
-  for (int j = 0; j < LoadOffsets<D>::kLoads; ++j) {
-    if (once) global_to_lds16_sbase_nt_at(base, off[j], lds + 1024 * j);
-    else global_to_lds16_sbase_at(base, off[j], lds + 1024 * j);
-  }
+// The loads of one slab: m0 is set once, each instruction's offset counts for the global
+// and for the LDS address (global_to_lds16 in mfma_tile.h says why this is asm).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+template <int D, bool ONCE>
+__device__ __forceinline__ void load_slab(const char *base, const unsigned (&off)[D / 32],
+                                          unsigned lds) {
+  const unsigned m0 = __builtin_amdgcn_readfirstlane(lds);
+  if constexpr (D == 64 && ONCE)
+    asm volatile(
+        "s_mov_b32 m0, %3\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %0, %2 nt\n\t"
+        "global_load_lds_dwordx4 %1, %2 offset:1024 nt"
+        ::"v"(off[0]), "v"(off[1]), "s"(base), "s"(m0) : "memory", "m0");
+  else if constexpr (D == 64)
+    asm volatile(
+        "s_mov_b32 m0, %3\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %0, %2\n\t"
+        "global_load_lds_dwordx4 %1, %2 offset:1024"
+        ::"v"(off[0]), "v"(off[1]), "s"(base), "s"(m0) : "memory", "m0");
+  else if constexpr (ONCE)
+    asm volatile(
+        "s_mov_b32 m0, %5\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %0, %4 nt\n\t"
+        "global_load_lds_dwordx4 %1, %4 offset:1024 nt\n\t"
+        "global_load_lds_dwordx4 %2, %4 offset:2048 nt\n\t"
+        "global_load_lds_dwordx4 %3, %4 offset:3072 nt"
+        ::"v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base), "s"(m0)
+        : "memory", "m0");
+  else
+    asm volatile(
+        "s_mov_b32 m0, %5\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %0, %4\n\t"
+        "global_load_lds_dwordx4 %1, %4 offset:1024\n\t"
+        "global_load_lds_dwordx4 %2, %4 offset:2048\n\t"
+        "global_load_lds_dwordx4 %3, %4 offset:3072"
+        ::"v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base), "s"(m0)
+        : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 // ---- results -------------------------------------------------------------------------
 
@@ -424,7 +509,7 @@ __device__ __forceinline__ floatx2 fetch2(const float *p) {
 template <typename T>
 __device__ __forceinline__ T *out_row(const AttendPagedParams &p, int t0, int kvh, int row,
                                       int head_dim) {
-  const int token = row / p.group;
+  const int token = token_of(p, row);
   const int head = kvh * p.group + row - token * p.group;
   return static_cast<T *>(p.out) +
          (static_cast<int64_t>(t0 + token) * p.heads + head) * head_dim;
@@ -440,15 +525,6 @@ __device__ __forceinline__ void store4(T *dst, const floatx4 &x) {
 }
 
 // ---- items ----------------------------------------------------------------------------
-
-struct Item {
-  int t0, n, p0;     // packed tokens and the first one's position
-  int kvh;
-  int kt0, kt1;      // key tiles of this share
-  int end;           // keys the item sees (the last token's)
-  int slot;          // partial slot, -1: the whole item
-  uniform_table table;
-};
 
 __device__ __forceinline__ void block_barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -490,42 +566,50 @@ __device__ __forceinline__ void wide_item(const AttendPagedParams &p, const Item
                                           unsigned ring) {
   constexpr int kTileBytes = kTileKeys * D * 2;
   constexpr int kStages = kRingBytes / (2 * kTileBytes);
-  constexpr int kLoads = 2 * LoadOffsets<D>::kLoads;  // a wave's loads per tile
+  constexpr int kLoads = 2 * (D / 32);  // a wave's loads per tile
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 5;
   const int rows = it.n * p.group;
   const int row = 32 * wave + (lane & 31);
   const FragOffsetsD<D> fo = frag_offsets_d<D>(lane);
-  const LoadOffsets<D> lo = load_offsets<D>(lane);
+  const LoadOffsets<D, false> lo = load_offsets<D, false>(lane);
   const frag_t<T> ones = ones_selector<T>(lane);
-  Rows<T, D> r;
-  load_queries<T, D>(p, it.t0, it.n, it.p0, it.kvh, row, g, r);
-  clear_rows<T, D>(r);
   // Positions of the wave's first and last query.
-  const int first_pos = it.p0 + min(32 * wave, rows - 1) / p.group;
-  const int last_pos = it.p0 + min(32 * wave + 31, rows - 1) / p.group;
+  const int first_pos = it.p0 + token_of(p, min(32 * wave, rows - 1));
+  const int last_pos = it.p0 + token_of(p, min(32 * wave + 31, rows - 1));
   const bool has_rows = 32 * wave < rows;
 
-  // Wave w loads rows [16 w, +16) of each tile's K and V.
+  // Wave w loads rows [16 w, +16) of each tile's K and V. A tile's page ids are read one
+  // step before its loads leave; `absent` queues its masks until it is used.
+  struct Ids {
+    PageIds<kTileKeys / 16> all;
+    PageIds<1> own;
+  };
+  auto ids_of = [&](int kt) {
+    return Ids{page_ids<kTileKeys / 16>(p, it, kt * kTileKeys),
+               page_ids<1>(p, it, kt * kTileKeys + 16 * wave)};
+  };
+  unsigned absent[kStages];
+  Ids ids = ids_of(it.kt0);
   auto issue = [&](int kt) {
     const int stage = (kt - it.kt0) % kStages;
-    const Slab s = slab_of(p, it.table, it.kvh, kt * kTileKeys + 16 * wave, it.end);
+    const Slabs<1> slab = slabs_of<D>(p, it, ids.own, kt * kTileKeys + 16 * wave);
     const unsigned at = ring + stage * 2 * kTileBytes + 16 * wave * D * 2;
-    load_slab<D>(p.k_pages, s.at, lo.k, at, false);
-    load_slab<D>(p.v_pages, s.at, lo.v, at + kTileBytes, false);
+    load_slab<D, false>(it.k + slab.at[0], lo.k, at);
+    load_slab<D, false>(it.v + slab.at[0], lo.v, at + kTileBytes);
   };
-  auto absent_rows = [&](int kt) {
-    unsigned absent = 0;
 #pragma unroll
-    for (int i = 0; i < kTileKeys / 16; ++i)
-      absent |= slab_of(p, it.table, it.kvh, kt * kTileKeys + 16 * i, it.end).absent ? 1u << i : 0u;
-    return absent;
-  };
-
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i)
+  for (int i = 0; i < kStages - 1; ++i) {
+    absent[i] = absent_of(p, ids.all);
     if (it.kt0 + i < it.kt1) issue(it.kt0 + i);
+    ids = ids_of(it.kt0 + i + 1);
+  }
+  Rows<T, D> r;
+  const T *q = query_row<T>(p, it, min(row, rows - 1), r.pos);  // rows past the last repeat it
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) r.q[s] = load_query<T>(p, q + (D / 2) * g + 8 * s);
+  clear_rows<T, D>(r);
   for (int kt = it.kt0; kt < it.kt1; ++kt) {
     // Tile kt has landed once at most the later tiles' loads are outstanding.
     const int later = min(kStages - 2, it.kt1 - 1 - kt);
@@ -533,23 +617,27 @@ __device__ __forceinline__ void wide_item(const AttendPagedParams &p, const Item
     else if (kStages > 2 && later == 1) wait_loads<kLoads>();
     else wait_loads<0>();
     block_barrier();
+    absent[kStages - 1] = absent_of(p, ids.all);
     if (kt + kStages - 1 < it.kt1) issue(kt + kStages - 1);
+    ids = ids_of(kt + kStages);
     const unsigned k_tile = ring + ((kt - it.kt0) % kStages) * 2 * kTileBytes;
     const unsigned v_tile = k_tile + kTileBytes;
     const int key0 = kt * kTileKeys;
-    const unsigned absent = absent_rows(kt);
-    if (absent != 0 || key0 + kTileKeys > it.end) {
-      clear_v<D>(v_tile, kTileKeys, it.end - key0, absent, threadIdx.x, kThreads);
+    const unsigned gone = absent[0];
+#pragma unroll
+    for (int i = 0; i + 1 < kStages; ++i) absent[i] = absent[i + 1];
+    if (gone != 0 || key0 + kTileKeys > it.end) {
+      clear_v<D>(v_tile, kTileKeys, it.end - key0, gone, threadIdx.x, kThreads);
       block_barrier();
     }
     if (!has_rows || last_pos < key0) continue;
     floatx16 s[2];
-    frag_t<T> hi[4], none[4];
+    frag_t<T> weights[4];
     scores<T, D, 2>(k_tile, fo, r, s);
-    if (absent != 0 || first_pos < key0 + kTileKeys - 1 || key0 + kTileKeys > it.end)
-      hide<2>(s, min(r.pos, it.end - 1) - key0 - 4 * g, absent);
-    weigh<T, D, 2, false>(s, p.c, r, hi, none);
-    accumulate<T, D, 2, false>(v_tile, fo, ones, hi, none, r);
+    if (gone != 0 || first_pos < key0 + kTileKeys - 1 || key0 + kTileKeys > it.end)
+      hide<2>(s, min(r.pos, it.end - 1) - key0 - 4 * g, gone);
+    weigh<T, D, 2>(s, p.c, r, weights);
+    accumulate<T, D, 2>(v_tile, fo, ones, weights, r);
   }
   block_barrier();  // the ring may be filled for the next item
 
@@ -602,83 +690,178 @@ __device__ __forceinline__ void join_wide(const AttendPagedParams &p, const Item
   write_rows<T, D>(p, it, row, lane >> 5, o, l);
 }
 
-template <typename T, int D>
+// Narrow items run on v_mfma_f32_16x16x32, with NQ groups of 16 query rows: with the
+// 32-row products a group of 7 query heads paid for 32 rows of softmax, 2600 cycles per
+// 64-key tile of head_dim 64 against XX.
+// Lane l: query l % 16 of a group, g = l / 16. S^T of 16 keys: A = K rows (k-step s, lane g:
+// dims [32 s + 8 g, +8)), B = Q^T alike; the lane gets keys 4 g + j. O^T of 16 dims: A = V^T,
+// k index 8 g + 4 part + e standing for key 16 part + 4 g + e of a 32-key step, which is how
+// the lane's own weights of two 16-key blocks lie; the lane gets dims 4 g + j.
+template <typename T, int D, int NQ>
 __device__ __forceinline__ void narrow_item(const AttendPagedParams &p, const Item &it,
                                             unsigned ring, float *exchange, float *exchange_ml) {
   constexpr int kKeys = 4096 / D;  // keys of a wave's 8 KiB tile
-  constexpr int KB = kKeys / 32;
+  constexpr int KB = kKeys / 16;
   constexpr int kTileBytes = 8192;
   constexpr int kLoads = 8;        // load instructions per tile
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int g = lane >> 5;
+  const int col = lane & 15, g = lane >> 4;
   const int rows = it.n * p.group;
-  const FragOffsetsD<D> fo = frag_offsets_d<D>(lane);
-  const LoadOffsets<D> lo = load_offsets<D>(lane);
-  const frag_t<T> ones = ones_selector<T>(lane);
+  const LoadOffsets<D, true> lo = load_offsets<D, true>(lane);
   const unsigned k_tile = ring + wave * 2 * kTileBytes, v_tile = k_tile + kTileBytes;
   const int stop = min(it.end, it.kt1 * kTileKeys);
-  auto issue = [&](const void *pages, const unsigned (&off)[LoadOffsets<D>::kLoads], unsigned lds,
-                   int key0) {
-    unsigned absent = 0;
+  typedef PageIds<kKeys / 16> Ids;
+  typedef Slabs<kKeys / 16> WaveSlabs;
+  auto issue = [&](const WaveSlabs &slabs, const char *base, const unsigned (&off)[D / 32],
+                   unsigned lds) {
 #pragma unroll
-    for (int i = 0; i < kKeys / 16; ++i) {
-      const Slab s = slab_of(p, it.table, it.kvh, key0 + 16 * i, it.end);
-      absent |= s.absent ? 1u << i : 0u;
-      load_slab<D>(pages, s.at, off, lds + 16 * i * D * 2, true);
-    }
-    return absent;
+    for (int i = 0; i < kKeys / 16; ++i)
+      load_slab<D, true>(base + slabs.at[i], off, lds + 16 * i * D * 2);
   };
   int key0 = it.kt0 * kTileKeys + wave * kKeys;
-  unsigned absent = 0;
+  Ids ids = page_ids<kKeys / 16>(p, it, key0);
   if (key0 < stop) {
-    absent = issue(p.k_pages, lo.k, k_tile, key0);
-    issue(p.v_pages, lo.v, v_tile, key0);
+    const WaveSlabs slabs = slabs_of<D>(p, it, ids, key0);
+    issue(slabs, it.k, lo.k, k_tile);
+    issue(slabs, it.v, lo.v, v_tile);
   }
-  Rows<T, D> r;
-  load_queries<T, D>(p, it.t0, it.n, it.p0, it.kvh, lane & 31, g, r);
-  clear_rows<T, D>(r);
+  frag_t<T> q[NQ][D / 32];
+  int pos[NQ];
+#pragma unroll
+  for (int i = 0; i < NQ; ++i) {
+    const T *row = query_row<T>(p, it, min(16 * i + col, rows - 1), pos[i]);
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) q[i][s] = load_query<T>(p, row + 32 * s + 8 * g);
+  }
+  // Fragment offsets, in halves: K chunk 4 s + g of row `col`; V rows 4 g + col / 4, dims
+  // 16 db + 4 (col % 4).
+  int fk[D / 32], fv[D / 16];
+#pragma unroll
+  for (int s = 0; s < D / 32; ++s) fk[s] = col * D + (((4 * s + g) ^ k_swz_d<D>(col)) << 3);
+  const int v_row = 4 * g + (col >> 2);
+#pragma unroll
+  for (int db = 0; db < D / 16; ++db)
+    fv[db] = v_row * D + (((2 * db + ((col >> 1) & 1)) ^ group_v_swz<D>(v_row)) << 3) + 4 * (col & 1);
+
+  floatx4 o[NQ][D / 16];
+  float m[NQ], l[NQ];  // l: the lane's share of the row sum
+#pragma unroll
+  for (int i = 0; i < NQ; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db) o[i][db] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
   for (; key0 < stop; key0 += kWaves * kKeys) {
+    typedef __attribute__((address_space(3))) const frag_t<T> lds_frag;
     const int next = key0 + kWaves * kKeys;
+    const unsigned absent = absent_of(p, ids);
+    ids = page_ids<kKeys / 16>(p, it, next);
     // Loads leave in the order K, V, K, V: at most the 8 of V are younger than K's.
     wait_loads<kLoads>();
-    floatx16 s[KB];
-    frag_t<T> hi[2 * KB], low[2 * KB];
-    scores<T, D, KB>(k_tile, fo, r, s);
+    floatx4 s[NQ][KB];
+#pragma unroll
+    for (int i = 0; i < NQ; ++i)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) s[i][kb] = floatx4{0.f, 0.f, 0.f, 0.f};
+    const unsigned k_base = uniform_lds_u(k_tile);
+#pragma unroll
+    for (int st = 0; st < D / 32; ++st) {
+      lds_half *at = opaque_lds_at(k_base, fk[st]);
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const frag_t<T> k = *reinterpret_cast<lds_frag *>(at + kb * 16 * D);
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) s[i][kb] = Frag<T>::mm16(k, q[i][st], s[i][kb]);
+      }
+    }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K is read before it is overwritten
-    unsigned next_absent = 0;
-    if (next < stop) next_absent = issue(p.k_pages, lo.k, k_tile, next);
-    if (absent != 0 || it.p0 < key0 + kKeys - 1 || key0 + kKeys > it.end)
-      hide<KB>(s, min(r.pos, it.end - 1) - key0 - 4 * g, absent);
-    weigh<T, D, KB, true>(s, p.c, r, hi, low);
+    const WaveSlabs slabs = slabs_of<D>(p, it, ids, next);
+    if (next < stop) issue(slabs, it.k, lo.k, k_tile);
+    if (absent != 0 || it.p0 < key0 + kKeys - 1 || key0 + kKeys > it.end) {
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        const int lim = min(pos[i], it.end - 1) - key0 - 4 * g;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            s[i][kb][j] =
+                (16 * kb + j <= lim && !((absent >> kb) & 1)) ? s[i][kb][j] : -INFINITY;
+      }
+    }
+    // Weights, split into two parts of the type, and the bound m (as in weigh).
+    frag_t<T> hi[NQ][KB / 2], low[NQ][KB / 2];
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mx = fmaxf(mx, s[i][kb][j]);
+      mx = max_lane_groups(mx) * p.c;
+      if (__builtin_amdgcn_ballot_w64(mx > m[i] + 8.0f) != 0) {
+        const float top = fmaxf(m[i], mx);
+        const float alpha = top == -INFINITY ? 1.0f : fast_exp2(m[i] - top);
+        m[i] = top;
+        l[i] *= alpha;
+#pragma unroll
+        for (int db = 0; db < D / 16; ++db) o[i][db] *= alpha;
+      }
+      const float bound = m[i] == -INFINITY ? 0.0f : m[i];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float w = fast_exp2(__builtin_fmaf(s[i][kb][j], p.c, -bound));
+          const T h = static_cast<T>(w);
+          hi[i][kb / 2][4 * (kb % 2) + j] = h;
+          low[i][kb / 2][4 * (kb % 2) + j] = static_cast<T>(w - static_cast<float>(h));
+          l[i] += w;
+        }
+    }
     if (next < stop) wait_loads<kLoads>();
     else wait_loads<0>();
     if (absent != 0 || key0 + kKeys > it.end) {
       clear_v<D>(v_tile, kKeys, it.end - key0, absent, lane, kWave);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
-    accumulate<T, D, KB, true>(v_tile, fo, ones, hi, low, r);
+    const unsigned v_base = uniform_lds_u(v_tile);
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db) {
+      lds_half *at = opaque_lds_at(v_base, fv[db]);
+#pragma unroll
+      for (int ks = 0; ks < KB / 2; ++ks) {
+        const frag_t<T> v = read_v<T>(at + 32 * ks * D, at + (32 * ks + 16) * D);
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+          o[i][db] = Frag<T>::mm16(v, hi[i][ks], o[i][db]);
+          o[i][db] = Frag<T>::mm16(v, low[i][ks], o[i][db]);
+        }
+      }
+    }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (next < stop) issue(p.v_pages, lo.v, v_tile, next);
-    absent = next_absent;
+    if (next < stop) issue(slabs, it.v, lo.v, v_tile);
   }
 
   // Join the four waves' states. Row r's dims lie in LDS as 16-byte pieces,
   // piece j at j ^ (r & 15).
   block_barrier();  // every wave is done with its tiles
-  const int row = lane & 31;
-  if (row < rows) {
-    float *x = exchange + (wave * kNarrowRows + row) * D;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i)
+  for (int i = 0; i < NQ; ++i) {
+    const int row = 16 * i + col;
+    float sum = l[i] + __shfl_xor(l[i], 16);
+    sum += __shfl_xor(sum, 32);
+    if (row < rows) {
+      float *x = exchange + (wave * kNarrowRows + row) * D;
 #pragma unroll
-      for (int a = 0; a < 4; ++a) {
-        const floatx4 o = {r.o[i][4 * a], r.o[i][4 * a + 1], r.o[i][4 * a + 2], r.o[i][4 * a + 3]};
-        *reinterpret_cast<floatx4 *>(x + 4 * ((8 * i + 2 * a + g) ^ (row & 15))) = o;
+      for (int db = 0; db < D / 16; ++db)
+        *reinterpret_cast<floatx4 *>(x + 4 * ((4 * db + g) ^ col)) = o[i][db];
+      if (g == 0) {
+        exchange_ml[2 * (wave * kNarrowRows + row)] = m[i];
+        exchange_ml[2 * (wave * kNarrowRows + row) + 1] = sum;
       }
-    if (g == 0) {
-      exchange_ml[2 * (wave * kNarrowRows + row)] = r.m;
-      exchange_ml[2 * (wave * kNarrowRows + row) + 1] = r.l[0];
     }
   }
   block_barrier();
@@ -754,75 +937,87 @@ template <typename T, int D>
 __global__ __launch_bounds__(kThreads, 2) void attend_paged_kernel(const AttendPagedParams p) {
   __shared__ __align__(1024) unsigned char ring_mem[kRingBytes];
   __shared__ __align__(16) float ml_mem[2 * kWaves * kNarrowRows];
-  __shared__ int64_t wave_weight[kWaves];
-  __shared__ Border borders[2];
   __shared__ int arrived;
 
+  // One word of each 64-byte line of the arguments, read together: the lines' misses
+  // (their first use in a launch) overlap instead of following one another.
+  {
+    const auto *args = (uniform_ints)__builtin_amdgcn_kernarg_segment_ptr();
+    int touched = 0;
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(AttendPagedParams); i += 64) touched ^= args[i / 4];
+    asm volatile("" ::"s"(touched));
+  }
   const int tid = static_cast<int>(threadIdx.x);
+  const int lane = tid & 63;
   const int n_blocks = static_cast<int>(gridDim.x);
+  const uniform_ints bounds = uniform_at(p.cu_tokens), lens = uniform_at(p.seq_lens);
+  // Packed rows that belong to no sequence: [0, head) and [tail, tokens).
+  const int head = min(max(bounds[0], 0), p.tokens);
+  const int tail = min(max(bounds[p.batch], 0), p.tokens);
 
-  // Every block sums the sequences' weights and finds its share's two borders.
-  const int per = (p.batch + kThreads - 1) / kThreads;
-  const int b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
-  int64_t mine = 0;
+  // Every wave sums the sequences' weights (lane l takes `per` of them) and finds its
+  // block's two borders: no exchange between waves, and scalar code from there on.
+  const int per = (p.batch + kWave - 1) / kWave;
+  int mine = 0;
   Seq s = {0, 0, 0};
-  for (int b = b0; b < b1; ++b) {
-    s = load_seq(p, b);
-    const Tiles t = tiles_of(p, s.n);
+  for (int i = 0; i < per; ++i) {
+    const int b = lane * per + i;
+    if (b >= p.batch) break;
+    s = load_seq(p, p.cu_tokens, p.seq_lens, b);
+    const Tiles t = tiles_of<false>(p, s.n);
     mine += weight_before(p, s, t, t.count) * p.kv_heads;
   }
-  int64_t before = mine;  // inclusive sum over the wave
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) {
-    const int64_t x = __shfl_up(before, d);
-    if ((tid & 63) >= d) before += x;
-  }
-  if ((tid & 63) == 63) wave_weight[tid >> 6] = before;
-  if (tid < 2) borders[tid].b = p.batch;
-  __syncthreads();
-  int64_t total = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    if (w < (tid >> 6)) before += wave_weight[w];
-    total += wave_weight[w];
-  }
-  before -= mine;
-  const int64_t share = max(floor_div(total, n_blocks) + 1, static_cast<int64_t>(kMinShareKeys));
+  const int upto = wave_prefix(mine);
+  const int total = __builtin_amdgcn_readlane(upto, kWave - 1);
+  // share * n_blocks > total, whatever the reciprocal's last bit.
+  const int share = max(static_cast<int>(__umulhi(total, p.blocks_inv)) + 2, p.min_share);
   // Neighbouring shares read the same keys, so they go to one XCD (blocks are
-  // dealt to the 8 XCDs in turn).
-  const int active = static_cast<int>(floor_div(total, share)) + 1;
-  const int per_xcd = (min(active, n_blocks) + 7) / 8;
+  // dealt to the 8 XCDs in turn). Any estimate of the shares in use is right here.
+  const int active = static_cast<int>(static_cast<float>(total) *
+                                      __builtin_amdgcn_rcpf(static_cast<float>(share))) + 1;
+  const int per_xcd =
+      (__builtin_amdgcn_readfirstlane(min(active, n_blocks)) + 7) / 8;
   const int blk = static_cast<int>(blockIdx.x);
-  const int w = blk < 8 * per_xcd ? (blk & 7) * per_xcd + (blk >> 3) : blk;
-#pragma unroll 1
-  for (int side = 0; side < 2; ++side) {
-    const int64_t at = (w + side) * share;
-    if (at < before || at >= before + mine) continue;
-    int64_t from = before;
-    for (int b = b0; b < b1; ++b) {
-      if (per > 1) s = load_seq(p, b);
-      const Tiles t = tiles_of(p, s.n);
-      const int64_t whole = weight_before(p, s, t, t.count);
-      if (at < from + whole * p.kv_heads) {
-        borders[side] = border_in(p, s, t, b, whole, from, at);
-        break;
-      }
-      from += whole * p.kv_heads;
+  const int w = blk < 8 * per_xcd && 8 * per_xcd <= n_blocks ? (blk & 7) * per_xcd + (blk >> 3) : blk;
+  // Even lanes compute the share's first border, odd lanes its end, in one pass.
+  const int at0 = w * share, at1 = at0 + share;
+  const int owner0 = __builtin_popcountll(__builtin_amdgcn_ballot_w64(upto <= at0));
+  const int owner1 = __builtin_popcountll(__builtin_amdgcn_ballot_w64(upto <= at1));
+  const int owner = (lane & 1) ? owner1 : owner0;
+  const int at = (lane & 1) ? at1 : at0;
+  Border border;
+  border.from = __shfl(upto - mine, owner & 63);
+  border.b = owner * per;
+  if (per == 1) {
+    border.s.t0 = __shfl(s.t0, owner & 63);
+    border.s.n = __shfl(s.n, owner & 63);
+    border.s.p0 = __shfl(s.p0, owner & 63);
+  } else if (owner < kWave) {
+    for (;; ++border.b) {  // the owner's sequences
+      border.s = load_seq(p, p.cu_tokens, p.seq_lens, border.b);
+      const Tiles t = tiles_of<false>(p, border.s.n);
+      const int weight = weight_before(p, border.s, t, t.count) * p.kv_heads;
+      if (at < border.from + weight || border.b + 1 >= p.batch) break;
+      border.from += weight;
     }
   }
-  __syncthreads();
-  auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
-  int b = uniform(borders[0].b), kvh = uniform(borders[0].kvh), tile = uniform(borders[0].tile);
-  int kt = uniform(borders[0].kt);
-  s.t0 = uniform(borders[0].s.t0);
-  s.n = uniform(borders[0].s.n);
-  s.p0 = uniform(borders[0].s.p0);
-  int64_t from = borders[0].from;
-  const int end_b = uniform(borders[1].b), end_kvh = uniform(borders[1].kvh);
-  const int end_tile = uniform(borders[1].tile), end_kt = uniform(borders[1].kt);
+  if (owner < kWave) place_border(p, tiles_of<false>(p, border.s.n), at, border);
+  else border.b = p.batch;
+  struct { int b, kvh, tile, kt; } end;
+  int b = __builtin_amdgcn_readlane(border.b, 0), kvh = __builtin_amdgcn_readlane(border.kvh, 0);
+  int tile = __builtin_amdgcn_readlane(border.tile, 0), kt = __builtin_amdgcn_readlane(border.kt, 0);
+  int from = __builtin_amdgcn_readlane(border.from, 0);
+  s.t0 = __builtin_amdgcn_readlane(border.s.t0, 0);
+  s.n = __builtin_amdgcn_readlane(border.s.n, 0);
+  s.p0 = __builtin_amdgcn_readlane(border.s.p0, 0);
+  end.b = __builtin_amdgcn_readlane(border.b, 1);
+  end.kvh = __builtin_amdgcn_readlane(border.kvh, 1);
+  end.tile = __builtin_amdgcn_readlane(border.tile, 1);
+  end.kt = __builtin_amdgcn_readlane(border.kt, 1);
 
   const unsigned ring = lds_addr(ring_mem);
-  Tiles t = tiles_of(p, s.n);
+  Tiles t = tiles_of<true>(p, s.n);
   while (b < p.batch) {
     if (tile >= t.count) {  // next K/V head or sequence
       tile = 0;
@@ -832,41 +1027,42 @@ __global__ __launch_bounds__(kThreads, 2) void attend_paged_kernel(const AttendP
         kvh = 0;
         ++b;
         if (b >= p.batch) break;
-        s = load_seq(p, b);
-        s.t0 = uniform(s.t0);
-        s.n = uniform(s.n);
-        s.p0 = uniform(s.p0);
-        t = tiles_of(p, s.n);
+        s = load_seq(p, bounds, lens, b);
+        t = tiles_of<true>(p, s.n);
       }
-      if (b > end_b) break;
+      if (b > end.b) break;
       continue;
     }
-    const bool last = b == end_b && kvh == end_kvh && tile == end_tile;
+    const bool last = b == end.b && kvh == end.kvh && tile == end.tile;
     Item it;
     it.end = key_end(p, s, t, tile);
     const int tiles = key_tiles(it.end);
     it.kt0 = kt;
-    it.kt1 = last ? min(end_kt, tiles) : tiles;
+    it.kt1 = last ? min(end.kt, tiles) : tiles;
     it.t0 = s.t0 + tile * t.tokens;
     it.n = min(t.tokens, s.n - tile * t.tokens);
     it.p0 = s.p0 + tile * t.tokens;
     it.kvh = kvh;
-    it.table = (uniform_table)(reinterpret_cast<uintptr_t>(
-        p.page_table + static_cast<int64_t>(b) * p.max_pages));
+    const uint64_t head_at = static_cast<uint64_t>(kvh) * p.head_bytes;
+    it.k = static_cast<const char *>(p.k_pages) + head_at;
+    it.v = static_cast<const char *>(p.v_pages) + head_at;
+    it.table = uniform_at(p.page_table + static_cast<int64_t>(b) * p.max_pages);
     // A whole item (also one that sees no key) is written out; a part leaves a partial.
-    const bool whole = it.kt0 == 0 && it.kt1 == tiles && !(last && end_kt < tiles) &&
+    const bool whole = it.kt0 == 0 && it.kt1 == tiles && !(last && end.kt < tiles) &&
                        !(last && tiles == 0);
     if (whole || it.kt1 > it.kt0) {
       it.slot = whole ? -1 : 2 * w + (it.kt0 == 0 ? 1 : 0);
-      if (it.n * p.group <= kNarrowRows)
-        narrow_item<T, D>(p, it, ring, reinterpret_cast<float *>(ring_mem), ml_mem);
+      if (it.n * p.group <= 16)
+        narrow_item<T, D, 1>(p, it, ring, reinterpret_cast<float *>(ring_mem), ml_mem);
+      else if (it.n * p.group <= kNarrowRows)
+        narrow_item<T, D, 2>(p, it, ring, reinterpret_cast<float *>(ring_mem), ml_mem);
       else
         wide_item<T, D>(p, it, ring);
     }
     if (!whole && it.kt1 > it.kt0) {
-      const int64_t x0 = from + kvh * weight_before(p, s, t, t.count) + weight_before(p, s, t, tile);
-      const int64_t x1 = x0 + weight_before(p, s, t, tile + 1) - weight_before(p, s, t, tile);
-      const Pieces pc = pieces_of(x0, x1, tiles, share);
+      const int x0 = from + kvh * weight_before(p, s, t, t.count) + weight_before(p, s, t, tile);
+      const int x1 = x0 + weight_before(p, s, t, tile + 1) - weight_before(p, s, t, tile);
+      const Pieces pc = pieces_of(p, t, x0, x1, tiles, share);
       // The partial is stored before it is counted; the block that counts last sets the
       // counter back to zero for the next call.
       wait_loads<0>();
@@ -892,13 +1088,12 @@ __global__ __launch_bounds__(kThreads, 2) void attend_paged_kernel(const AttendP
   }
 
   // Outputs of packed rows that belong to no sequence are zero.
-  const int lo = min(max(p.cu_tokens[0], 0), p.tokens);
-  const int hi = min(max(p.cu_tokens[p.batch], 0), p.tokens);
+  if (head + p.tokens - tail <= 0) return;
   const int64_t per_row = static_cast<int64_t>(p.heads) * (D / 8);
-  const int64_t outside = (static_cast<int64_t>(lo) + p.tokens - hi) * per_row;
+  const int64_t outside = (static_cast<int64_t>(head) + p.tokens - tail) * per_row;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + tid; i < outside;
        i += static_cast<int64_t>(n_blocks) * kThreads) {
-    const int64_t at = i < lo * per_row ? i : i + (static_cast<int64_t>(hi) - lo) * per_row;
+    const int64_t at = i < head * per_row ? i : i + (static_cast<int64_t>(tail) - head) * per_row;
     const uint4 zero = {0, 0, 0, 0};
     static_cast<uint4 *>(p.out)[at] = zero;
   }
@@ -943,6 +1138,21 @@ int launch_attend_paged(AttendPagedParams p, bool bf16, int head_dim, float scal
   p.group = p.heads / p.kv_heads;
   p.slot_rows = slot_rows_of(p.tokens, p.group);
   p.capacity = p.max_pages << p.page_shift;
+  p.wide_tokens = kWideRows / p.group;
+  p.narrow_tokens = kNarrowRows / p.group;
+  p.head_bytes = static_cast<unsigned>((head_dim * 2) << p.page_shift);
+  p.page_bytes = p.head_bytes * static_cast<unsigned>(p.kv_heads);
+  p.narrow_step = kWaves * (4096 / head_dim) / kTileKeys;
+  p.wide_inv = 1.0f / static_cast<float>(p.wide_tokens);
+  p.group_inv = (65536 + p.group - 1) / p.group;
+  // Weight of any batch of this many tokens and sequences.
+  const double tiles = static_cast<double>(p.tokens) / p.wide_tokens + p.batch;
+  const double most =
+      tiles * p.kv_heads * (2.0 + p.capacity + kItemKeys + p.tokens + 2.0 * p.wide_tokens);
+  p.unit = 0;
+  while (most / static_cast<double>(1u << p.unit) + tiles * p.kv_heads > 1e9 && p.unit < 30) ++p.unit;
+  p.blocks_inv = static_cast<unsigned>(0xffffffffu / static_cast<unsigned>(n_blocks));
+  p.min_share = (kMinShareKeys >> p.unit) + 1;
   // A negative scale negates q (exactly), so that the row bound is a maximum; a
   // zero one becomes the least that keeps a hidden key's -inf (-inf * 0 is NaN).
   p.negate = scale < 0.f;
