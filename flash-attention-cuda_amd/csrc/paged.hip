@@ -52,9 +52,11 @@ constexpr int kTileKeys = 64;     // keys per tile of a wide item, and the unit 
 constexpr int kWideRows = 128;    // query rows of a wide item
 constexpr int kNarrowRows = 32;   // most query rows of a narrow item
 constexpr int kRingBytes = 64 * 1024;
-constexpr int kItemKeys = 128;    // an item's fixed cost, in keys
-constexpr int kMinShareKeys = 256;  // least weight of a share
-constexpr int kSnapTiles = 1;     // borders this close to an item's end move there
+constexpr int kItemKeys = 320;    // an item's fixed cost, in keys, when there are many
+constexpr int kFewItemKeys = 512; // and when blocks are to spare: no block takes two items
+constexpr int kMinShareKeys = 512;  // least weight of a share
+constexpr int kWideStep = 2;      // borders inside wide items lie at multiples of this many tiles
+constexpr int kWholeSteps = 4;    // items of at most this many steps are never cut
 
 template <typename T>
 struct Frag;
@@ -126,7 +128,7 @@ __device__ __forceinline__ Tiles tiles_of(const AttendPagedParams &p, int n) {
   Tiles t;
   const bool narrow = n <= p.narrow_tokens;
   t.tokens = narrow ? max(n, 1) : p.wide_tokens;
-  t.step = narrow ? p.narrow_step : 1;
+  t.step = narrow ? p.narrow_step : kWideStep;
   // n / wide_tokens, rounded up, by its reciprocal (n < 2^24: exact in fp32 to within one).
   int q = static_cast<int>(static_cast<float>(n) * p.wide_inv);
   q += q * p.wide_tokens < n;
@@ -141,16 +143,20 @@ __device__ __forceinline__ int key_end(const AttendPagedParams &p, const Seq &s,
   // p0 + n <= 2^30 + 2^24
   return min(max(s.p0 + min(s.n, (tile + 1) * t.tokens), 0), p.capacity);
 }
-// Weight of tiles [0, tile) of one K/V head: the keys each tile sees (taken as
-// if the last tile were whole) plus a fixed cost per item, in units of 2^unit
-// keys, at least one per item. The host picks the unit that keeps a batch's
-// weight within 30 bits (one key, but for batches of 10^9 keys and more).
-__device__ __forceinline__ int weight_before(const AttendPagedParams &p, const Seq &s,
-                                             const Tiles &t, int tile) {
-  const int each = min(max(s.p0, 0), p.capacity) + kItemKeys;
+// Keys that tiles [0, tile) of one K/V head see (taken as if the last tile were whole), in
+// units of 2^unit. The host picks the unit that keeps a batch's weight within 30 bits (one
+// key, but for batches of 10^9 keys and more).
+__device__ __forceinline__ int keys_before(const AttendPagedParams &p, const Seq &s,
+                                           const Tiles &t, int tile) {
+  const int each = min(max(s.p0, 0), p.capacity);
   const int64_t keys = static_cast<int64_t>(tile) * each +
                        (static_cast<int64_t>(tile) * (tile + 1) >> 1) * t.tokens;
-  return tile + static_cast<int>(keys >> p.unit);
+  return static_cast<int>(keys >> p.unit);
+}
+// Weight of those tiles: their keys and `item` units for each.
+__device__ __forceinline__ int weight_before(const AttendPagedParams &p, const Seq &s,
+                                             const Tiles &t, int item, int tile) {
+  return tile * item + keys_before(p, s, t, tile);
 }
 
 // Key tiles of an item.
@@ -173,26 +179,28 @@ struct Border {
 };
 
 // The border at weight `at` inside sequence b (0 <= at - from < H_kv * whole).
-__device__ __forceinline__ void place_border(const AttendPagedParams &p, const Tiles &t, int at,
-                                             Border &r) {
-  const int whole = weight_before(p, r.s, t, t.count);
+__device__ __forceinline__ void place_border(const AttendPagedParams &p, const Tiles &t, int item,
+                                             int at, Border &r) {
+  const int whole = weight_before(p, r.s, t, item, t.count);
   at -= r.from;
   r.kvh = floor_div(at, whole);
   at -= r.kvh * whole;
   int lo = 0, hi = t.count;  // the last tile whose weight_before is <= at
   while (hi - lo > 1) {
     const int mid = (lo + hi) / 2;
-    if (weight_before(p, r.s, t, mid) <= at) lo = mid;
+    if (weight_before(p, r.s, t, item, mid) <= at) lo = mid;
     else hi = mid;
   }
   r.tile = lo;
   const int tiles = key_tiles(key_end(p, r.s, t, lo));
-  const int64_t in =
-      (static_cast<int64_t>(at - weight_before(p, r.s, t, lo)) << p.unit) - kItemKeys;
-  r.kt = static_cast<int>(min(max(in, int64_t{0}) / kTileKeys, static_cast<int64_t>(tiles)));
-  // A border close to an item's end moves there: a partial costs more than the keys it balances.
+  const int in = max(at - weight_before(p, r.s, t, item, lo) - item, 0);
+  r.kt = static_cast<int>(min((static_cast<int64_t>(in) << p.unit) / kTileKeys,
+                              static_cast<int64_t>(tiles)));
   r.kt -= r.kt % t.step;
-  if (r.kt > tiles - kSnapTiles) r.kt = tiles;
+  // A border close to an item's end moves there, and none cuts a short item: a partial
+  // costs more than the keys it balances.
+  if (tiles <= kWholeSteps * t.step) r.kt = 0;
+  else if (r.kt > tiles - t.step) r.kt = tiles;
 }
 
 // The shares that an item of `tiles` key tiles at weights [x0, x1) is cut into: the
@@ -204,13 +212,13 @@ struct Pieces {
 __device__ __forceinline__ int ceil_units(const AttendPagedParams &p, int64_t keys) {
   return static_cast<int>((keys + (int64_t{1} << p.unit) - 1) >> p.unit);
 }
-__device__ __forceinline__ Pieces pieces_of(const AttendPagedParams &p, const Tiles &t, int x0,
-                                            int x1, int tiles, int share) {
+__device__ __forceinline__ Pieces pieces_of(const AttendPagedParams &p, const Tiles &t,
+                                            int item, int x0, int x1, int tiles, int share) {
   Pieces r;
-  const int start = x0 + ceil_units(p, kItemKeys + t.step * kTileKeys);
+  const int start = x0 + item + ceil_units(p, t.step * kTileKeys);
   r.first = __builtin_amdgcn_readfirstlane(floor_div(start + share - 1, share));
-  const int64_t beyond = tiles - kSnapTiles - (tiles - kSnapTiles) % t.step + t.step;
-  const int stop = min(x1, x0 + ceil_units(p, kItemKeys + beyond * kTileKeys));
+  const int64_t beyond = tiles - tiles % t.step;
+  const int stop = min(x1, x0 + item + ceil_units(p, beyond * kTileKeys));
   r.count = __builtin_amdgcn_readfirstlane(floor_div(stop + share - 1, share)) - r.first + 1;
   return r;
 }
@@ -708,7 +716,6 @@ __device__ __forceinline__ void narrow_item(const AttendPagedParams &p, const It
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
   const int rows = it.n * p.group;
-  const LoadOffsets<D, true> lo = load_offsets<D, true>(lane);
   const unsigned k_tile = ring + wave * 2 * kTileBytes, v_tile = k_tile + kTileBytes;
   const int stop = min(it.end, it.kt1 * kTileKeys);
   typedef PageIds<kKeys / 16> Ids;
@@ -721,6 +728,7 @@ __device__ __forceinline__ void narrow_item(const AttendPagedParams &p, const It
   };
   int key0 = it.kt0 * kTileKeys + wave * kKeys;
   Ids ids = page_ids<kKeys / 16>(p, it, key0);
+  const LoadOffsets<D, true> lo = load_offsets<D, true>(lane);
   if (key0 < stop) {
     const WaveSlabs slabs = slabs_of<D>(p, it, ids, key0);
     issue(slabs, it.k, lo.k, k_tile);
@@ -895,8 +903,8 @@ __device__ __forceinline__ void narrow_item(const AttendPagedParams &p, const It
   block_barrier();  // the exchange may be overwritten
 }
 
-// Joins a narrow item's pieces, first to last, and writes its rows. Eight pieces' loads are
-// in flight at a time.
+// Joins a narrow item's pieces, first to last, and writes its rows. Eight pieces' loads
+// are in flight at a time.
 template <typename T, int D>
 __device__ __forceinline__ void join_narrow(const AttendPagedParams &p, const Item &it,
                                             const Pieces &pc) {
@@ -917,14 +925,21 @@ __device__ __forceinline__ void join_narrow(const AttendPagedParams &p, const It
         ml[j] = fetch2(part + p.slot_rows * D + 2 * row);
         x[j] = fetch2(part + row * D + at);
       }
+      float top = m;
+#pragma unroll
+      for (int j = 0; j < kDeep; ++j) top = fmaxf(top, ml[j][0]);
+      const float base = top == -INFINITY ? 0.f : top;
+      const float old = fast_exp2(m - base);
+      m = top;
+      l *= old;
+      o *= old;
 #pragma unroll
       for (int j = 0; j < kDeep; ++j) {
-        if (j0 + j >= pc.count || ml[j][0] == -INFINITY) continue;
-        const float top = fmaxf(m, ml[j][0]);
-        const float a = m == -INFINITY ? 0.f : fast_exp2(m - top), b = fast_exp2(ml[j][0] - top);
-        m = top;
-        l = l * a + ml[j][1] * b;
-        o = o * a + x[j] * b;
+        // A repeated last piece, or one whose keys the row does not see, counts for nothing.
+        const float a = j0 + j < pc.count ? fast_exp2(ml[j][0] - base) : 0.f;
+        l += a == 0.f ? 0.f : a * ml[j][1];
+        o[0] += a == 0.f ? 0.f : a * x[j][0];
+        o[1] += a == 0.f ? 0.f : a * x[j][1];
       }
     }
     const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
@@ -959,17 +974,25 @@ __global__ __launch_bounds__(kThreads, 2) void attend_paged_kernel(const AttendP
   // Every wave sums the sequences' weights (lane l takes `per` of them) and finds its
   // block's two borders: no exchange between waves, and scalar code from there on.
   const int per = (p.batch + kWave - 1) / kWave;
-  int mine = 0;
+  int mine = 0, my_items = 0;
   Seq s = {0, 0, 0};
   for (int i = 0; i < per; ++i) {
     const int b = lane * per + i;
     if (b >= p.batch) break;
     s = load_seq(p, p.cu_tokens, p.seq_lens, b);
     const Tiles t = tiles_of<false>(p, s.n);
-    mine += weight_before(p, s, t, t.count) * p.kv_heads;
+    mine += keys_before(p, s, t, t.count) * p.kv_heads;
+    my_items += t.count * p.kv_heads;
   }
-  const int upto = wave_prefix(mine);
-  const int total = __builtin_amdgcn_readlane(upto, kWave - 1);
+  const int keys_upto = wave_prefix(mine), items_upto = wave_prefix(my_items);
+  const int all_keys = __builtin_amdgcn_readlane(keys_upto, kWave - 1);
+  const int all_items = __builtin_amdgcn_readlane(items_upto, kWave - 1);
+  const int few = 1 + (kFewItemKeys >> p.unit);
+  const int item = all_items <= n_blocks && all_keys + all_items * few <= n_blocks * few
+                       ? few : 1 + (kItemKeys >> p.unit);
+  const int total = all_keys + all_items * item;
+  mine += my_items * item;
+  const int upto = keys_upto + items_upto * item;
   // share * n_blocks > total, whatever the reciprocal's last bit.
   const int share = max(static_cast<int>(__umulhi(total, p.blocks_inv)) + 2, p.min_share);
   // Neighbouring shares read the same keys, so they go to one XCD (blocks are
@@ -997,12 +1020,12 @@ __global__ __launch_bounds__(kThreads, 2) void attend_paged_kernel(const AttendP
     for (;; ++border.b) {  // the owner's sequences
       border.s = load_seq(p, p.cu_tokens, p.seq_lens, border.b);
       const Tiles t = tiles_of<false>(p, border.s.n);
-      const int weight = weight_before(p, border.s, t, t.count) * p.kv_heads;
+      const int weight = weight_before(p, border.s, t, item, t.count) * p.kv_heads;
       if (at < border.from + weight || border.b + 1 >= p.batch) break;
       border.from += weight;
     }
   }
-  if (owner < kWave) place_border(p, tiles_of<false>(p, border.s.n), at, border);
+  if (owner < kWave) place_border(p, tiles_of<false>(p, border.s.n), item, at, border);
   else border.b = p.batch;
   struct { int b, kvh, tile, kt; } end;
   int b = __builtin_amdgcn_readlane(border.b, 0), kvh = __builtin_amdgcn_readlane(border.kvh, 0);
@@ -1023,7 +1046,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend_paged_kernel(const AttendP
       tile = 0;
       kt = 0;
       if (t.count == 0 || ++kvh >= p.kv_heads) {
-        from += weight_before(p, s, t, t.count) * p.kv_heads;
+        from += weight_before(p, s, t, item, t.count) * p.kv_heads;
         kvh = 0;
         ++b;
         if (b >= p.batch) break;
@@ -1060,9 +1083,9 @@ __global__ __launch_bounds__(kThreads, 2) void attend_paged_kernel(const AttendP
         wide_item<T, D>(p, it, ring);
     }
     if (!whole && it.kt1 > it.kt0) {
-      const int x0 = from + kvh * weight_before(p, s, t, t.count) + weight_before(p, s, t, tile);
-      const int x1 = x0 + weight_before(p, s, t, tile + 1) - weight_before(p, s, t, tile);
-      const Pieces pc = pieces_of(p, t, x0, x1, tiles, share);
+      const int x0 = from + kvh * weight_before(p, s, t, item, t.count) + weight_before(p, s, t, item, tile);
+      const int x1 = x0 + weight_before(p, s, t, item, tile + 1) - weight_before(p, s, t, item, tile);
+      const Pieces pc = pieces_of(p, t, item, x0, x1, tiles, share);
       // The partial is stored before it is counted; the block that counts last sets the
       // counter back to zero for the next call.
       wait_loads<0>();
