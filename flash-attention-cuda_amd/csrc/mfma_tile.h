@@ -207,6 +207,20 @@ __device__ __forceinline__ FragOffsetsD<D> frag_offsets_d(int lane) {
 
 typedef __attribute__((address_space(3))) const _Float16 lds_half;
 
+// The lane index read afresh from the hardware (v_mbcnt, in volatile asm so
+// that the compiler cannot merge it with the kernel's first lane index). In
+// prefill.hip the code after the main loop (masked tail, verdict, epilogue) derives its
+// per-lane values from this instead of from values computed before the loop,
+// which the compiler otherwise keeps live across it: at 256 VGPRs they went
+// to scratch (5 per lane at head_dim 64, 11-15 at 128), each item stored and
+// reloaded them, and their write-backs were 2.5-3.4 MB of a C3 launch's HBM
+// writes (C3 46.2 -> 45.8 us, C2 full 27.1 -> 26.4 us without them).
+__device__ __forceinline__ int fresh_lane() {
+  int l;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
+  return l;
+}
+
 // A wave-uniform LDS byte address kept whole in an SGPR (so no constant part of
 // it is split off into a separate vector add).
 __device__ __forceinline__ unsigned uniform_lds_u(unsigned a) {

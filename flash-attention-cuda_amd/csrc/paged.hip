@@ -51,12 +51,25 @@ constexpr int kWaves = 4;
 constexpr int kTileKeys = 64;     // keys per tile of a wide item, and the unit of a share's border
 constexpr int kWideRows = 128;    // query rows of a wide item
 constexpr int kNarrowRows = 32;   // most query rows of a narrow item
-constexpr int kRingBytes = 64 * 1024;
+constexpr int kNarrowKeys = 32;   // keys of a narrow item's tile, of which each wave has its own
 constexpr int kItemKeys = 320;    // an item's fixed cost, in keys, when there are many
 constexpr int kFewItemKeys = 512; // and when blocks are to spare: no block takes two items
 constexpr int kMinShareKeys = 512;  // least weight of a share
 constexpr int kWideStep = 2;      // borders inside wide items lie at multiples of this many tiles
 constexpr int kWholeSteps = 4;    // items of at most this many steps are never cut
+
+// Blocks per CU and LDS for tiles per block, by head size. A head_dim 64 wave fits 168
+// VGPRs, so three blocks share a CU.
+template <int D>
+struct Geo;
+template <>
+struct Geo<64> {
+  static constexpr int kBlocks = 3, kRingBytes = 48 * 1024;
+};
+template <>
+struct Geo<128> {
+  static constexpr int kBlocks = 2, kRingBytes = 64 * 1024;
+};
 
 template <typename T>
 struct Frag;
@@ -236,11 +249,14 @@ __device__ __forceinline__ int wave_prefix(int x) {
 
 // A V^T operand from two transposed reads (four keys each) of a V tile.
 template <typename T>
-__device__ __forceinline__ frag_t<T> read_v(lds_half *first, lds_half *second) {
+__device__ __forceinline__ frag_t<T> read_v(unsigned tile, int first, int second) {
   typedef T t4 __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) short4v lds_short4;
-  const t4 a = __builtin_bit_cast(t4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)first));
-  const t4 b = __builtin_bit_cast(t4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)second));
+  auto read = [&](int off) {
+    return __builtin_bit_cast(t4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        reinterpret_cast<lds_short4 *>(static_cast<uintptr_t>(tile + 2u * off))));
+  };
+  const t4 a = read(first), b = read(second);
   return frag_t<T>{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
 
@@ -302,25 +318,46 @@ __device__ __forceinline__ frag_t<T> load_query(const AttendPagedParams &p, cons
 
 // ---- one tile of KB 32-key blocks: scores, softmax, products ------------------------
 
-// Scores of the tile at LDS byte address `tile`.
+// A 16-byte operand of an LDS tile, `off` halves (per lane) from its byte address.
+template <typename T>
+__device__ __forceinline__ frag_t<T> read_frag(unsigned tile, int off) {
+  typedef __attribute__((address_space(3))) const frag_t<T> lds_frag;
+  return *reinterpret_cast<lds_frag *>(static_cast<uintptr_t>(tile + 2u * off));
+}
+
+// All of a tile's K operands, read before the first product: a product that waits for its
+// own read costs the LDS latency each time (at XX).
 template <typename T, int D, int KB>
 __device__ __forceinline__ void scores(unsigned tile, const FragOffsetsD<D> &fo,
                                        const Rows<T, D> &r, floatx16 (&s)[KB]) {
-  typedef __attribute__((address_space(3))) const frag_t<T> lds_frag;
-  const unsigned base = uniform_lds_u(tile);
+  frag_t<T> k[D / 16][KB];
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) k[i][kb] = read_frag<T>(tile, fo.k[i] + kb * 32 * D);
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
     for (int a = 0; a < 16; ++a) s[kb][a] = 0.f;
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i) {
-    lds_half *at = opaque_lds_at(base, fo.k[i]);
+  for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      const frag_t<T> k = *reinterpret_cast<lds_frag *>(at + kb * 32 * D);
-      s[kb] = Frag<T>::mm(k, r.q[i], s[kb]);
-    }
-  }
+    for (int kb = 0; kb < KB; ++kb) s[kb] = Frag<T>::mm(k[i][kb], r.q[i], s[kb]);
+}
+
+// All of a tile's V^T operands; they land under the softmax.
+template <typename T, int D, int KB>
+struct ValueFrags {
+  frag_t<T> f[D / 32][2 * KB];
+};
+template <typename T, int D, int KB>
+__device__ __forceinline__ void read_values(unsigned tile, const FragOffsetsD<D> &fo,
+                                            ValueFrags<T, D, KB> &v) {
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int ks = 0; ks < 2 * KB; ++ks)
+      v.f[db][ks] = read_v<T>(tile, fo.v[db] + ks * 16 * D, fo.v[db] + (ks * 16 + 8) * D);
 }
 
 // Hides keys above `lim` (the lane's position less the tile's first key and the
@@ -368,18 +405,13 @@ __device__ __forceinline__ void weigh(floatx16 (&s)[KB], float c, Rows<T, D> &r,
 }
 
 template <typename T, int D, int KB>
-__device__ __forceinline__ void accumulate(unsigned tile, const FragOffsetsD<D> &fo,
-                                           const frag_t<T> &ones, const frag_t<T> (&w)[2 * KB],
-                                           Rows<T, D> &r) {
-  const unsigned base = uniform_lds_u(tile);
+__device__ __forceinline__ void accumulate(const ValueFrags<T, D, KB> &v, const frag_t<T> &ones,
+                                           const frag_t<T> (&w)[2 * KB], Rows<T, D> &r) {
 #pragma unroll
-  for (int ks = 0; ks < 2 * KB; ++ks) r.l = Frag<T>::mm16(ones, w[ks], r.l);
+  for (int ks = 0; ks < 2 * KB; ++ks) {
+    r.l = Frag<T>::mm16(ones, w[ks], r.l);
 #pragma unroll
-  for (int db = 0; db < D / 32; ++db) {
-    lds_half *at = opaque_lds_at(base, fo.v[db]);
-#pragma unroll
-    for (int ks = 0; ks < 2 * KB; ++ks)
-      r.o[db] = Frag<T>::mm(read_v<T>(at + ks * 16 * D, at + (ks * 16 + 8) * D), w[ks], r.o[db]);
+    for (int db = 0; db < D / 32; ++db) r.o[db] = Frag<T>::mm(v.f[db][ks], w[ks], r.o[db]);
   }
 }
 
@@ -573,9 +605,9 @@ template <typename T, int D>
 __device__ __forceinline__ void wide_item(const AttendPagedParams &p, const Item &it,
                                           unsigned ring) {
   constexpr int kTileBytes = kTileKeys * D * 2;
-  constexpr int kStages = kRingBytes / (2 * kTileBytes);
+  constexpr int kStages = Geo<D>::kRingBytes / (2 * kTileBytes);
   constexpr int kLoads = 2 * (D / 32);  // a wave's loads per tile
-  const int lane = threadIdx.x & 63;
+  const int lane = fresh_lane();  // per-lane offsets live in one kind of item only
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 5;
   const int rows = it.n * p.group;
@@ -645,7 +677,9 @@ __device__ __forceinline__ void wide_item(const AttendPagedParams &p, const Item
     if (gone != 0 || first_pos < key0 + kTileKeys - 1 || key0 + kTileKeys > it.end)
       hide<2>(s, min(r.pos, it.end - 1) - key0 - 4 * g, gone);
     weigh<T, D, 2>(s, p.c, r, weights);
-    accumulate<T, D, 2>(v_tile, fo, ones, weights, r);
+    ValueFrags<T, D, 2> v;
+    read_values<T, D, 2>(v_tile, fo, v);
+    accumulate<T, D, 2>(v, ones, weights, r);
   }
   block_barrier();  // the ring may be filled for the next item
 
@@ -668,7 +702,7 @@ __device__ __forceinline__ void wide_item(const AttendPagedParams &p, const Item
 template <typename T, int D>
 __device__ __forceinline__ void join_wide(const AttendPagedParams &p, const Item &it,
                                           const Pieces &pc) {
-  const int lane = threadIdx.x & 63;
+  const int lane = fresh_lane();  // per-lane offsets live in one kind of item only
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = 32 * wave + (lane & 31);
   if (32 * wave >= it.n * p.group) return;
@@ -708,11 +742,11 @@ __device__ __forceinline__ void join_wide(const AttendPagedParams &p, const Item
 template <typename T, int D, int NQ>
 __device__ __forceinline__ void narrow_item(const AttendPagedParams &p, const Item &it,
                                             unsigned ring, float *exchange, float *exchange_ml) {
-  constexpr int kKeys = 4096 / D;  // keys of a wave's 8 KiB tile
+  constexpr int kKeys = kNarrowKeys;
   constexpr int KB = kKeys / 16;
-  constexpr int kTileBytes = 8192;
-  constexpr int kLoads = 8;        // load instructions per tile
-  const int lane = threadIdx.x & 63;
+  constexpr int kTileBytes = kKeys * D * 2;
+  constexpr int kLoads = kTileBytes / 1024;  // load instructions per tile
+  const int lane = fresh_lane();  // per-lane offsets live in one kind of item only
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
   const int rows = it.n * p.group;
@@ -762,28 +796,27 @@ __device__ __forceinline__ void narrow_item(const AttendPagedParams &p, const It
     for (int db = 0; db < D / 16; ++db) o[i][db] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
   for (; key0 < stop; key0 += kWaves * kKeys) {
-    typedef __attribute__((address_space(3))) const frag_t<T> lds_frag;
     const int next = key0 + kWaves * kKeys;
     const unsigned absent = absent_of(p, ids);
     ids = page_ids<kKeys / 16>(p, it, next);
-    // Loads leave in the order K, V, K, V: at most the 8 of V are younger than K's.
+    // Loads leave in the order K, V, K, V: at most those of V are younger than K's.
     wait_loads<kLoads>();
     floatx4 s[NQ][KB];
 #pragma unroll
     for (int i = 0; i < NQ; ++i)
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) s[i][kb] = floatx4{0.f, 0.f, 0.f, 0.f};
-    const unsigned k_base = uniform_lds_u(k_tile);
+    frag_t<T> k[D / 32][KB];
 #pragma unroll
-    for (int st = 0; st < D / 32; ++st) {
-      lds_half *at = opaque_lds_at(k_base, fk[st]);
+    for (int st = 0; st < D / 32; ++st)
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        const frag_t<T> k = *reinterpret_cast<lds_frag *>(at + kb * 16 * D);
+      for (int kb = 0; kb < KB; ++kb) k[st][kb] = read_frag<T>(k_tile, fk[st] + kb * 16 * D);
+  #pragma unroll
+    for (int st = 0; st < D / 32; ++st)
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) s[i][kb] = Frag<T>::mm16(k, q[i][st], s[i][kb]);
-      }
-    }
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) s[i][kb] = Frag<T>::mm16(k[st][kb], q[i][st], s[i][kb]);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K is read before it is overwritten
     const WaveSlabs slabs = slabs_of<D>(p, it, ids, next);
     if (next < stop) issue(slabs, it.k, lo.k, k_tile);
@@ -835,20 +868,21 @@ __device__ __forceinline__ void narrow_item(const AttendPagedParams &p, const It
       clear_v<D>(v_tile, kKeys, it.end - key0, absent, lane, kWave);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
-    const unsigned v_base = uniform_lds_u(v_tile);
+    frag_t<T> v[D / 16][KB / 2];
 #pragma unroll
-    for (int db = 0; db < D / 16; ++db) {
-      lds_half *at = opaque_lds_at(v_base, fv[db]);
+    for (int db = 0; db < D / 16; ++db)
 #pragma unroll
-      for (int ks = 0; ks < KB / 2; ++ks) {
-        const frag_t<T> v = read_v<T>(at + 32 * ks * D, at + (32 * ks + 16) * D);
+      for (int ks = 0; ks < KB / 2; ++ks)
+        v[db][ks] = read_v<T>(v_tile, fv[db] + 32 * ks * D, fv[db] + (32 * ks + 16) * D);
+  #pragma unroll
+    for (int db = 0; db < D / 16; ++db)
+#pragma unroll
+      for (int ks = 0; ks < KB / 2; ++ks)
 #pragma unroll
         for (int i = 0; i < NQ; ++i) {
-          o[i][db] = Frag<T>::mm16(v, hi[i][ks], o[i][db]);
-          o[i][db] = Frag<T>::mm16(v, low[i][ks], o[i][db]);
+          o[i][db] = Frag<T>::mm16(v[db][ks], hi[i][ks], o[i][db]);
+          o[i][db] = Frag<T>::mm16(v[db][ks], low[i][ks], o[i][db]);
         }
-      }
-    }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (next < stop) issue(slabs, it.v, lo.v, v_tile);
   }
@@ -949,8 +983,8 @@ __device__ __forceinline__ void join_narrow(const AttendPagedParams &p, const It
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, 2) void attend_paged_kernel(const AttendPagedParams p) {
-  __shared__ __align__(1024) unsigned char ring_mem[kRingBytes];
+__global__ __launch_bounds__(kThreads, Geo<D>::kBlocks) void attend_paged_kernel(const AttendPagedParams p) {
+  __shared__ __align__(1024) unsigned char ring_mem[Geo<D>::kRingBytes];
   __shared__ __align__(16) float ml_mem[2 * kWaves * kNarrowRows];
   __shared__ int arrived;
 
@@ -1128,10 +1162,10 @@ __global__ void zero_counters_kernel(unsigned *counters, int n) {
   if (i < n) counters[i] = 0;
 }
 
-int attend_blocks() {
+int attend_blocks(int head_dim) {
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess) return 0;
-  return 2 * device_cu_count(dev);
+  return (head_dim == 64 ? Geo<64>::kBlocks : Geo<128>::kBlocks) * device_cu_count(dev);
 }
 int slot_rows_of(int tokens, int group) {
   return static_cast<int64_t>(tokens) * group <= kNarrowRows ? kNarrowRows : kWideRows;
@@ -1149,14 +1183,14 @@ size_t counter_bytes(size_t n) { return (n * sizeof(unsigned) + 255) / 256 * 256
 }  // namespace
 
 size_t attend_paged_workspace_bytes(int tokens, int group, int head_dim) {
-  const size_t n = static_cast<size_t>(attend_blocks());
+  const size_t n = static_cast<size_t>(attend_blocks(head_dim));
   return counter_bytes(n) +
          2 * n * slot_rows_of(tokens, group) * (static_cast<size_t>(head_dim) + 2) * sizeof(float);
 }
 
 int launch_attend_paged(AttendPagedParams p, bool bf16, int head_dim, float scale, void *workspace,
                         hipStream_t stream) {
-  const int n_blocks = attend_blocks();
+  const int n_blocks = attend_blocks(head_dim);
   if (n_blocks <= 0) return set_error(FA_ERR_HIP, "could not query the compute-unit count");
   p.group = p.heads / p.kv_heads;
   p.slot_rows = slot_rows_of(p.tokens, p.group);
@@ -1165,7 +1199,7 @@ int launch_attend_paged(AttendPagedParams p, bool bf16, int head_dim, float scal
   p.narrow_tokens = kNarrowRows / p.group;
   p.head_bytes = static_cast<unsigned>((head_dim * 2) << p.page_shift);
   p.page_bytes = p.head_bytes * static_cast<unsigned>(p.kv_heads);
-  p.narrow_step = kWaves * (4096 / head_dim) / kTileKeys;
+  p.narrow_step = kWaves * kNarrowKeys / kTileKeys;
   p.wide_inv = 1.0f / static_cast<float>(p.wide_tokens);
   p.group_inv = (65536 + p.group - 1) / p.group;
   // Weight of any batch of this many tokens and sequences.

@@ -221,20 +221,6 @@ struct Blk : Geo<D> {
   return *reinterpret_cast<const half8 *>(p);
 }
 
-// The lane index read afresh from the hardware (v_mbcnt, in volatile asm so
-// that the compiler cannot merge it with the kernel's first lane index). The
-// code after the main loop (masked tail, verdict, epilogue) derives its
-// per-lane values from this instead of from values computed before the loop,
-// which the compiler otherwise keeps live across it: at 256 VGPRs they went
-// to scratch (5 per lane at head_dim 64, 11-15 at 128), each item stored and
-// reloaded them, and their write-backs were 2.5-3.4 MB of a C3 launch's HBM
-// writes (C3 46.2 -> 45.8 us, C2 full 27.1 -> 26.4 us without them).
-__device__ __forceinline__ int fresh_lane() {
-  int l;
-  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
-  return l;
-}
-
 // head_dim 64 sums P rows on the matrix cores (rowsum_mfma); head_dim 128,
 // whose loop has no registers to spare, sums them with v_dot2_f32_f16 per
 // lane.
