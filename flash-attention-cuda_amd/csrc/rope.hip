@@ -18,6 +18,13 @@
 // Work per thread: 16 dims of a row, as two 16-byte pieces: 8 pairs (halves:
 // dims [8u, +8) and [R/2 + 8u, +8); interleaved: dims [16u, +16)), or 16 dims to
 // copy. The eight sines and cosines serve every head the thread loops over.
+//
+// What bounds it: HBM, or for a step's few rows the launch and its chain of loads (us per
+// call in a graph of calls; 5.14 TB/s copy rate):
+//   rope B8 H32 S4096 D128 bf16, 537 MB            110.5   (floor 104.5)
+//   rope_backward B4 H12 S4096 D64 bf16, 50 MB      10.3   (9.8)
+//   append 6144 tokens H32/8 D128 bf16, 151 MB      25.9   (29.4: part stays in the last cache)
+//   rope of one token 3.0, append of 32 tokens 3.4
 
 #include "fa_internal.h"
 
@@ -100,6 +107,17 @@ __device__ __forceinline__ void turn(typename Vec8<T>::type &x, typename Vec8<T>
   }
 }
 
+// Non-temporal stores do not claim L2 lines that the loads want. Append, whose rows go to
+// many pages: always (6144 tokens H32/8 D128 35.9 -> 25.9 us, few tokens alike). rope: where
+// the output passes kStreamBytes and so no cache keeps it for its reader (268 MB 116.7 ->
+// 110.5 us; 25 and 37 MB outputs 10.3 -> 10.6 and 14.2 -> 15.0, which keep plain stores).
+constexpr int64_t kStreamBytes = int64_t{128} << 20;
+template <bool STREAM, typename V>
+__device__ __forceinline__ void store_piece(V *p, const V &x) {
+  if constexpr (STREAM) __builtin_nontemporal_store(x, p);
+  else *p = x;
+}
+
 struct RopeParams {
   const void *x;
   void *out;
@@ -107,22 +125,22 @@ struct RopeParams {
   const double *inv_freq;
   int64_t x_batch, x_head, x_row;  // strides of x in elements
   int64_t pos_batch;               // stride of positions (0: one row for every sequence)
-  int64_t units;                   // batch * seq * head_dim / 16
+  unsigned units;                  // batch * seq * head_dim / 16, under 2^31
   int heads, seq, head_dim, rotary, heads_per_thread;
   float factor;
   bool interleaved, backward;
 };
 
-template <typename T>
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeParams p) {
   typedef typename Vec8<T>::type V;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kRopeThreads + threadIdx.x;
+  const unsigned i = blockIdx.x * kRopeThreads + threadIdx.x;
   if (i >= p.units) return;
-  const int per_row = p.head_dim / 16;
-  const int u = static_cast<int>(i % per_row);
-  const int64_t token = i / per_row;
-  const int64_t b = token / p.seq;
-  const int n = static_cast<int>(token - b * p.seq);
+  const int row_shift = p.head_dim == 64 ? 2 : 3;
+  const int u = static_cast<int>(i & ((1u << row_shift) - 1));
+  const unsigned token = i >> row_shift;
+  const int64_t b = token / static_cast<unsigned>(p.seq);
+  const int n = static_cast<int>(token - static_cast<unsigned>(b) * p.seq);
   const int h0 = static_cast<int>(blockIdx.y) * p.heads_per_thread;
   const int h1 = min(h0 + p.heads_per_thread, p.heads);
   const Piece at = piece_of(u, p.rotary, p.interleaved);
@@ -140,8 +158,8 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeParams p) 
     V a = *reinterpret_cast<const V *>(xr + at.first);
     V c = *reinterpret_cast<const V *>(xr + at.second);
     if (at.turned) turn<T>(a, c, t, p.interleaved);
-    *reinterpret_cast<V *>(out + at.first) = a;
-    *reinterpret_cast<V *>(out + at.second) = c;
+    store_piece<STREAM>(reinterpret_cast<V *>(out + at.first), a);
+    store_piece<STREAM>(reinterpret_cast<V *>(out + at.second), c);
   }
 }
 
@@ -164,12 +182,12 @@ __device__ __forceinline__ int sequence_of(const int32_t *__restrict__ bounds, i
 template <typename T>
 __global__ __launch_bounds__(kRopeThreads) void append_paged_kernel(const AppendPagedParams p) {
   typedef typename Vec8<T>::type V;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kRopeThreads + threadIdx.x;
-  const int per_row = p.head_dim / 16;
-  const int u = static_cast<int>(i % per_row);
-  const int64_t token = i / per_row;
-  if (token >= p.tokens) return;
-  const int t = static_cast<int>(token);
+  const unsigned i = blockIdx.x * kRopeThreads + threadIdx.x;
+  const int row_shift = p.head_dim == 64 ? 2 : 3;
+  const int u = static_cast<int>(i & ((1u << row_shift) - 1));
+  const int t = static_cast<int>(i >> row_shift);
+  if (t >= p.tokens) return;
+  const int64_t token = t;
   const Piece at = piece_of(u, p.rotary, p.interleaved);
   const int h0 = static_cast<int>(blockIdx.y) * p.heads_per_thread;
   const int h1 = min(h0 + p.heads_per_thread, p.q_heads + 2 * p.kv_heads);
@@ -211,18 +229,20 @@ __global__ __launch_bounds__(kRopeThreads) void append_paged_kernel(const Append
     V c = *reinterpret_cast<const V *>(src + at.second);
     if (vh < 0 && at.turned) turn<T>(a, c, turns, p.interleaved);
     if (!live) a = c = V{};  // a query row behind the last sequence
-    *reinterpret_cast<V *>(dst + at.first) = a;
-    *reinterpret_cast<V *>(dst + at.second) = c;
+    store_piece<true>(reinterpret_cast<V *>(dst + at.first), a);
+    store_piece<true>(reinterpret_cast<V *>(dst + at.second), c);
   }
 }
 
-// Heads one thread takes: up to 8 (8 sines and cosines cost as much as the
-// loads and stores of about 6 heads), fewer while the launch has under 2048
-// threads per CU.
+// Heads one thread takes: up to 8, since 8 sines and cosines cost as many instructions as
+// about 6 heads' loads, products and stores, fewer while the launch has under kFill threads
+// per CU (B2 H14 S1733 D64: 5.7 us at 2048, 5.2 at 512; 466 tokens of H32/8 D128: 7.9, 6.8,
+// and 9.2 at 128).
+constexpr int kFill = 512;
 int heads_per_thread(int64_t units, int heads) {
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess) dev = 0;
-  const int64_t want = static_cast<int64_t>(device_cu_count(dev)) * 2048;
+  const int64_t want = static_cast<int64_t>(device_cu_count(dev)) * kFill;
   int n = 8;
   while (n > 1 && units * ((heads + n - 1) / n) < want) n /= 2;
   return n;
@@ -243,7 +263,7 @@ int launch_rope(const void *x, void *out, const int32_t *positions, const double
   p.x_head = x_head;
   p.x_row = x_row;
   p.pos_batch = pos_batch;
-  p.units = static_cast<int64_t>(batch) * seq * (head_dim / 16);
+  p.units = static_cast<unsigned>(batch) * static_cast<unsigned>(seq) * (head_dim / 16);
   p.heads = heads;
   p.seq = seq;
   p.head_dim = head_dim;
@@ -254,8 +274,11 @@ int launch_rope(const void *x, void *out, const int32_t *positions, const double
   p.backward = backward;
   const dim3 grid(static_cast<unsigned>((p.units + kRopeThreads - 1) / kRopeThreads),
                   static_cast<unsigned>((heads + p.heads_per_thread - 1) / p.heads_per_thread));
-  if (bf16) hipLaunchKernelGGL(rope_kernel<__bf16>, grid, dim3(kRopeThreads), 0, stream, p);
-  else hipLaunchKernelGGL(rope_kernel<_Float16>, grid, dim3(kRopeThreads), 0, stream, p);
+  const bool stream_out =
+      static_cast<int64_t>(p.units) * heads * 16 * static_cast<int64_t>(sizeof(_Float16)) > kStreamBytes;
+  auto *kernel = bf16 ? (stream_out ? rope_kernel<__bf16, true> : rope_kernel<__bf16, false>)
+                      : (stream_out ? rope_kernel<_Float16, true> : rope_kernel<_Float16, false>);
+  hipLaunchKernelGGL(kernel, grid, dim3(kRopeThreads), 0, stream, p);
   return check_hip(hipGetLastError(), "rope_kernel launch");
 }
 
