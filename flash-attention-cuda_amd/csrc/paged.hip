@@ -108,6 +108,16 @@ __device__ __forceinline__ frag_t<T> ones_selector(int lane) {
   return s;
 }
 
+// The kernel's arguments where the launch put them. An item reads them anew through a pointer
+// that the compiler cannot see through (`anew`): kept in scalar registers for the whole
+// kernel, they and what is derived from them went to VGPR lanes and back.
+typedef const __attribute__((address_space(4))) AttendPagedParams &ParamsRef;
+typedef const __attribute__((address_space(4))) AttendPagedParams *ParamsPtr;
+__device__ __forceinline__ ParamsRef anew(ParamsPtr p) {
+  asm volatile("" : "+s"(p));
+  return *p;
+}
+
 // ---- sequences, items and shares ------------------------------------------------
 
 typedef const __attribute__((address_space(4))) int32_t *uniform_ints;  // read with scalar loads
@@ -120,7 +130,7 @@ struct Seq {
   int t0, n, p0;
 };
 template <typename Ints>
-__device__ __forceinline__ Seq load_seq(const AttendPagedParams &p, Ints bounds, Ints lens, int b) {
+__device__ __forceinline__ Seq load_seq(ParamsRef p, Ints bounds, Ints lens, int b) {
   const int lo = bounds[b], hi = bounds[b + 1];
   Seq s;
   s.t0 = min(max(lo, 0), p.tokens);
@@ -137,7 +147,7 @@ struct Tiles {
   int step;  // borders inside its items lie at multiples of this many key tiles
 };
 template <bool SCALAR>  // n is the wave's, not the lane's
-__device__ __forceinline__ Tiles tiles_of(const AttendPagedParams &p, int n) {
+__device__ __forceinline__ Tiles tiles_of(ParamsRef p, int n) {
   Tiles t;
   const bool narrow = n <= p.narrow_tokens;
   t.tokens = narrow ? max(n, 1) : p.wide_tokens;
@@ -151,7 +161,7 @@ __device__ __forceinline__ Tiles tiles_of(const AttendPagedParams &p, int n) {
   return t;
 }
 // Keys the last token of a tile sees.
-__device__ __forceinline__ int key_end(const AttendPagedParams &p, const Seq &s, const Tiles &t,
+__device__ __forceinline__ int key_end(ParamsRef p, const Seq &s, const Tiles &t,
                                        int tile) {
   // p0 + n <= 2^30 + 2^24
   return min(max(s.p0 + min(s.n, (tile + 1) * t.tokens), 0), p.capacity);
@@ -159,7 +169,7 @@ __device__ __forceinline__ int key_end(const AttendPagedParams &p, const Seq &s,
 // Keys that tiles [0, tile) of one K/V head see (taken as if the last tile were whole), in
 // units of 2^unit. The host picks the unit that keeps a batch's weight within 30 bits (one
 // key, but for batches of 10^9 keys and more).
-__device__ __forceinline__ int keys_before(const AttendPagedParams &p, const Seq &s,
+__device__ __forceinline__ int keys_before(ParamsRef p, const Seq &s,
                                            const Tiles &t, int tile) {
   const int each = min(max(s.p0, 0), p.capacity);
   const int64_t keys = static_cast<int64_t>(tile) * each +
@@ -167,7 +177,7 @@ __device__ __forceinline__ int keys_before(const AttendPagedParams &p, const Seq
   return static_cast<int>(keys >> p.unit);
 }
 // Weight of those tiles: their keys and `item` units for each.
-__device__ __forceinline__ int weight_before(const AttendPagedParams &p, const Seq &s,
+__device__ __forceinline__ int weight_before(ParamsRef p, const Seq &s,
                                              const Tiles &t, int item, int tile) {
   return tile * item + keys_before(p, s, t, tile);
 }
@@ -192,7 +202,7 @@ struct Border {
 };
 
 // The border at weight `at` inside sequence b (0 <= at - from < H_kv * whole).
-__device__ __forceinline__ void place_border(const AttendPagedParams &p, const Tiles &t, int item,
+__device__ __forceinline__ void place_border(ParamsRef p, const Tiles &t, int item,
                                              int at, Border &r) {
   const int whole = weight_before(p, r.s, t, item, t.count);
   at -= r.from;
@@ -222,12 +232,13 @@ __device__ __forceinline__ void place_border(const AttendPagedParams &p, const T
 struct Pieces {
   int first, count;
 };
-__device__ __forceinline__ int ceil_units(const AttendPagedParams &p, int64_t keys) {
+__device__ __forceinline__ int ceil_units(ParamsRef p, int64_t keys) {
   return static_cast<int>((keys + (int64_t{1} << p.unit) - 1) >> p.unit);
 }
-__device__ __forceinline__ Pieces pieces_of(const AttendPagedParams &p, const Tiles &t,
+__device__ __forceinline__ Pieces pieces_of(ParamsRef p, const Tiles &t,
                                             int item, int x0, int x1, int tiles, int share) {
   Pieces r;
+  asm volatile("" : "+s"(share));  // its reciprocal is taken here, not kept from the prologue
   const int start = x0 + item + ceil_units(p, t.step * kTileKeys);
   r.first = __builtin_amdgcn_readfirstlane(floor_div(start + share - 1, share));
   const int64_t beyond = tiles - tiles % t.step;
@@ -284,7 +295,7 @@ __device__ __forceinline__ void clear_rows(Rows<T, D> &r) {
 
 // row / group for row < 128, by the host's ceil(2^16 / group): exact, the product is over
 // by less than 128 / 2^16 < 1 / group.
-__device__ __forceinline__ int token_of(const AttendPagedParams &p, int row) {
+__device__ __forceinline__ int token_of(ParamsRef p, int row) {
   return (row * p.group_inv) >> 16;
 }
 
@@ -294,13 +305,14 @@ struct Item {
   int kt0, kt1;      // key tiles of this share
   int end;           // keys the item sees (the last token's)
   int slot;          // partial slot, -1: the whole item
+  int wave;          // the calling wave's index in its block
   uniform_ints table;
   const char *k, *v;  // the K/V head's rows of page 0
 };
 
 // An item's query row, and its position.
 template <typename T>
-__device__ __forceinline__ const T *query_row(const AttendPagedParams &p, const Item &it, int row,
+__device__ __forceinline__ const T *query_row(ParamsRef p, const Item &it, int row,
                                               int &pos) {
   const int token = token_of(p, row);
   const int head = it.kvh * p.group + row - token * p.group;
@@ -309,7 +321,7 @@ __device__ __forceinline__ const T *query_row(const AttendPagedParams &p, const 
          static_cast<int64_t>(head) * p.q_head;
 }
 template <typename T>
-__device__ __forceinline__ frag_t<T> load_query(const AttendPagedParams &p, const T *q) {
+__device__ __forceinline__ frag_t<T> load_query(ParamsRef p, const T *q) {
   const unsigned flip = p.negate ? 0x80008000u : 0u;  // a negative scale: -q, exactly
   uint4 x = *reinterpret_cast<const uint4 *>(q);
   x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
@@ -415,6 +427,74 @@ __device__ __forceinline__ void accumulate(const ValueFrags<T, D, KB> &v, const 
   }
 }
 
+// x[l] + x[l ^ 32], and x[l] + x[l ^ 16] + x[l ^ 32] + x[l ^ 48], for every lane (VALU only,
+// asm as in max_lane_pair, mfma_tile.h).
+__device__ __forceinline__ float sum_lane_pair(float x) {
+  float a = x, b = x;
+  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 0\n\tv_add_f32 %0, %0, %1"
+               : "+v"(a), "+v"(b));
+  return a;
+}
+__device__ __forceinline__ float sum_lane_groups(float x) {
+  float a = sum_lane_pair(x), b = a;
+  asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 0\n\tv_add_f32 %0, %0, %1"
+               : "+v"(a), "+v"(b));
+  return a;
+}
+__device__ __forceinline__ bool is_finite(float x) { return fabsf(x) < INFINITY; }
+
+// `x` with the keys past `lim` cleared. Element e is key offset STRIDE (e / 4) + e % 4 from
+// the lane's first. (By bit masks: 8 compares per operand would need more scalar registers
+// than there are.)
+template <typename T, int STRIDE>
+__device__ __forceinline__ frag_t<T> keys_up_to(const frag_t<T> &x, int lim) {
+  uint4 b = __builtin_bit_cast(uint4, x);
+  auto keep = [lim](unsigned bits, int key) {  // elements `key` and `key` + 1
+    const int low = (key - 1 - lim) >> 31, high = (key - lim) >> 31;
+    return bits & static_cast<unsigned>((low & 0xffff) | (high & ~0xffff));
+  };
+  b.x = keep(b.x, 0);
+  b.y = keep(b.y, 2);
+  b.z = keep(b.z, STRIDE);
+  b.w = keep(b.w, STRIDE + 2);
+  return __builtin_bit_cast(frag_t<T>, b);
+}
+
+// accumulate for rows that must not meet what they do not see (careful passes). The sum of
+// the weights is taken lane by lane: the selector of the fast pass multiplies the weights
+// of the query 16 columns on by zero, so a NaN there would reach this row. In a masked
+// tile (`seen`) the products run once per position among the wave's rows, with the keys
+// past that position cleared, and the rows there take the result.
+template <typename T, int D, int KB>
+__device__ __forceinline__ void accumulate_seen(unsigned tile, const FragOffsetsD<D> &fo,
+                                                const frag_t<T> (&w)[2 * KB], bool seen,
+                                                int first_key, Rows<T, D> &r) {
+  float sum = 0.f;
+#pragma unroll
+  for (int ks = 0; ks < 2 * KB; ++ks)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += static_cast<float>(w[ks][e]);
+  r.l[0] += sum_lane_pair(sum);
+#pragma unroll 1
+  for (uint64_t todo = ~uint64_t{0}; todo != 0;) {
+    const int pos = seen ? __builtin_amdgcn_readlane(r.pos, __builtin_ctzll(todo)) : 0x7fffffff;
+    todo &= seen ? ~__builtin_amdgcn_ballot_w64(r.pos == pos) : 0;
+#pragma unroll
+    for (int ks = 0; ks < 2 * KB; ++ks) {
+      const int lim = pos - first_key - 16 * ks;
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db) {
+        const frag_t<T> v = keys_up_to<T, 8>(
+            read_v<T>(tile, fo.v[db] + ks * 16 * D, fo.v[db] + (ks * 16 + 8) * D), lim);
+        const floatx16 o = Frag<T>::mm(v, w[ks], r.o[db]);
+#pragma unroll
+        for (int a = 0; a < 16; ++a) r.o[db][a] = r.pos == pos || !seen ? o[a] : r.o[db][a];
+        __builtin_amdgcn_sched_barrier(0);  // one operand at a time: this path is rare
+      }
+    }
+  }
+}
+
 // ---- pages --------------------------------------------------------------------------
 
 // Page ids of the N 16-key slabs from `key` on: N scalar loads, in flight together. Keys
@@ -424,19 +504,19 @@ struct PageIds {
   int id[N];
 };
 template <int N>
-__device__ __forceinline__ PageIds<N> page_ids(const AttendPagedParams &p, const Item &it,
+__device__ __forceinline__ PageIds<N> page_ids(ParamsRef p, const Item &it,
                                                int key) {
   PageIds<N> r;
 #pragma unroll
   for (int i = 0; i < N; ++i) r.id[i] = it.table[min(key + 16 * i, it.end - 1) >> p.page_shift];
   return r;
 }
-__device__ __forceinline__ bool is_absent(const AttendPagedParams &p, int id) {
+__device__ __forceinline__ bool is_absent(ParamsRef p, int id) {
   return static_cast<unsigned>(id) >= static_cast<unsigned>(p.num_pages);
 }
 // Bit i: slab i lies on a page outside the pool.
 template <int N>
-__device__ __forceinline__ unsigned absent_of(const AttendPagedParams &p, const PageIds<N> &ids) {
+__device__ __forceinline__ unsigned absent_of(ParamsRef p, const PageIds<N> &ids) {
   unsigned absent = 0;
 #pragma unroll
   for (int i = 0; i < N; ++i) absent |= is_absent(p, ids.id[i]) ? 1u << i : 0u;
@@ -449,7 +529,7 @@ struct Slabs {
   uint64_t at[N];
 };
 template <int D, int N>
-__device__ __forceinline__ Slabs<N> slabs_of(const AttendPagedParams &p, const Item &it,
+__device__ __forceinline__ Slabs<N> slabs_of(ParamsRef p, const Item &it,
                                              const PageIds<N> &ids, int key) {
   Slabs<N> r;
 #pragma unroll
@@ -526,7 +606,7 @@ __device__ __forceinline__ void load_slab(const char *base, const unsigned (&off
 
 // Partial of a share. Narrow items: rows of D floats, then (m, l) pairs from slot_rows D
 // on. Wide items: each wave's accumulators as (pair of elements, lane), then the pairs.
-__device__ __forceinline__ float *partial_of(const AttendPagedParams &p, int slot, int head_dim) {
+__device__ __forceinline__ float *partial_of(ParamsRef p, int slot, int head_dim) {
   return p.partials + static_cast<int64_t>(slot) * p.slot_rows * (head_dim + 2);
 }
 
@@ -547,7 +627,7 @@ __device__ __forceinline__ floatx2 fetch2(const float *p) {
 }
 
 template <typename T>
-__device__ __forceinline__ T *out_row(const AttendPagedParams &p, int t0, int kvh, int row,
+__device__ __forceinline__ T *out_row(ParamsRef p, int t0, int kvh, int row,
                                       int head_dim) {
   const int token = token_of(p, row);
   const int head = kvh * p.group + row - token * p.group;
@@ -586,7 +666,7 @@ __device__ __forceinline__ void clear_v(unsigned tile, int rows, int from, unsig
 
 // Normalises and stores the lane's half of its query row.
 template <typename T, int D>
-__device__ __forceinline__ void write_rows(const AttendPagedParams &p, const Item &it, int row,
+__device__ __forceinline__ void write_rows(ParamsRef p, const Item &it, int row,
                                            int g, const floatx16 (&o)[D / 32], float l) {
   if (row >= it.n * p.group) return;
   const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;  // NaN stays NaN
@@ -601,14 +681,17 @@ __device__ __forceinline__ void write_rows(const AttendPagedParams &p, const Ite
     }
 }
 
-template <typename T, int D>
-__device__ __forceinline__ void wide_item(const AttendPagedParams &p, const Item &it,
-                                          unsigned ring) {
+// One pass over a wide item's keys. Its weights of zero hide no infinity or NaN (0 * inf): the
+// CAREFUL pass, which takes about twice as long, runs again over an item that the first
+// one left with a result that is not finite.
+template <typename T, int D, bool CAREFUL>
+__device__ __forceinline__ void wide_pass(ParamsRef p, const Item &it,
+                                          unsigned ring, Rows<T, D> &r) {
   constexpr int kTileBytes = kTileKeys * D * 2;
   constexpr int kStages = Geo<D>::kRingBytes / (2 * kTileBytes);
   constexpr int kLoads = 2 * (D / 32);  // a wave's loads per tile
   const int lane = fresh_lane();  // per-lane offsets live in one kind of item only
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = it.wave;
   const int g = lane >> 5;
   const int rows = it.n * p.group;
   const int row = 32 * wave + (lane & 31);
@@ -645,7 +728,6 @@ __device__ __forceinline__ void wide_item(const AttendPagedParams &p, const Item
     if (it.kt0 + i < it.kt1) issue(it.kt0 + i);
     ids = ids_of(it.kt0 + i + 1);
   }
-  Rows<T, D> r;
   const T *q = query_row<T>(p, it, min(row, rows - 1), r.pos);  // rows past the last repeat it
 #pragma unroll
   for (int s = 0; s < D / 16; ++s) r.q[s] = load_query<T>(p, q + (D / 2) * g + 8 * s);
@@ -667,43 +749,75 @@ __device__ __forceinline__ void wide_item(const AttendPagedParams &p, const Item
 #pragma unroll
     for (int i = 0; i + 1 < kStages; ++i) absent[i] = absent[i + 1];
     if (gone != 0 || key0 + kTileKeys > it.end) {
-      clear_v<D>(v_tile, kTileKeys, it.end - key0, gone, threadIdx.x, kThreads);
+      clear_v<D>(v_tile, kTileKeys, it.end - key0, gone, 64 * wave + fresh_lane(), kThreads);
       block_barrier();
     }
     if (!has_rows || last_pos < key0) continue;
     floatx16 s[2];
     frag_t<T> weights[4];
     scores<T, D, 2>(k_tile, fo, r, s);
-    if (gone != 0 || first_pos < key0 + kTileKeys - 1 || key0 + kTileKeys > it.end)
+    const bool masked =
+        gone != 0 || first_pos < key0 + kTileKeys - 1 || key0 + kTileKeys > it.end;
+    if (masked)
       hide<2>(s, min(r.pos, it.end - 1) - key0 - 4 * g, gone);
     weigh<T, D, 2>(s, p.c, r, weights);
-    ValueFrags<T, D, 2> v;
-    read_values<T, D, 2>(v_tile, fo, v);
-    accumulate<T, D, 2>(v, ones, weights, r);
+    if constexpr (CAREFUL) {
+      accumulate_seen<T, D, 2>(v_tile, fo, weights, masked, key0 + 4 * g, r);
+    } else {
+      ValueFrags<T, D, 2> v;
+      read_values<T, D, 2>(v_tile, fo, v);
+      accumulate<T, D, 2>(v, ones, weights, r);
+    }
   }
-  block_barrier();  // the ring may be filled for the next item
+  block_barrier();  // the ring may be filled again
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void wide_item(ParamsRef p, const Item &it,
+                                          unsigned ring, int *votes, Rows<T, D> &r) {
+  const int wave = it.wave;
+  const bool has_rows = 32 * wave < it.n * p.group;
+  wide_pass<T, D, false>(p, it, ring, r);
+  // Sums of finite values below 2^100 are finite, so one sum tells for all of them.
+  float probe = r.l[0];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int a = 0; a < 16; ++a) probe += r.o[i][a];
+  const bool lost = __builtin_amdgcn_ballot_w64(has_rows && !is_finite(probe)) != 0;
+  if (fresh_lane() == 0) votes[wave] = lost;
+  block_barrier();
+  if (votes[0] | votes[1] | votes[2] | votes[3]) wide_pass<T, D, true>(p, it, ring, r);
 
   if (!has_rows) return;
+  const int out_lane = fresh_lane(), out_row = 32 * wave + (out_lane & 31);
   if (it.slot < 0) {
-    write_rows<T, D>(p, it, row, g, r.o, r.l[0]);
+    write_rows<T, D>(p, it, out_row, out_lane >> 5, r.o, r.l[0]);
   } else {
-    float *part = partial_of(p, it.slot, D) + wave * (32 * D) + 2 * lane;
+    float *part = partial_of(p, it.slot, D) + wave * (32 * D) + 2 * out_lane;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
       for (int a = 0; a < 8; ++a)
         publish2(part + (8 * i + a) * 128, r.o[i][2 * a], r.o[i][2 * a + 1]);
-    if (g == 0)
-      publish2(partial_of(p, it.slot, D) + kWideRows * D + 2 * row, r.m, r.l[0]);
+    if (out_lane < 32)
+      publish2(partial_of(p, it.slot, D) + kWideRows * D + 2 * out_row, r.m, r.l[0]);
   }
 }
 
-// Joins a wide item's pieces, first to last, and writes its rows.
+// o a + x b, both products rounded: the same bits wherever x came from.
+__device__ __forceinline__ float fold(float o, float a, float x, float b) {
+#pragma clang fp contract(off)
+  return o * a + x * b;
+}
+
+// Joins a wide item's pieces, first to last, and writes its rows. Piece `own` is the
+// block's, still in its registers; the others come from the workspace, at ~5 thousand
+// cycles each (32 KiB at head_dim 64, past the L2).
 template <typename T, int D>
-__device__ __forceinline__ void join_wide(const AttendPagedParams &p, const Item &it,
-                                          const Pieces &pc) {
-  const int lane = fresh_lane();  // per-lane offsets live in one kind of item only
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+__device__ __forceinline__ void join_wide(ParamsRef p, const Item &it,
+                                          const Pieces &pc, int own, const Rows<T, D> &r) {
+  const int lane = fresh_lane(), wave = it.wave;
   const int row = 32 * wave + (lane & 31);
   if (32 * wave >= it.n * p.group) return;
   float m = -INFINITY, l = 0.f;
@@ -713,20 +827,27 @@ __device__ __forceinline__ void join_wide(const AttendPagedParams &p, const Item
 #pragma unroll
     for (int a = 0; a < 16; ++a) o[i][a] = 0.f;
   for (int j = 0; j < pc.count; ++j) {
-    const float *part = partial_of(p, 2 * (pc.first + j - 1) + (j == 0 ? 1 : 0), D);
-    const floatx2 ml = fetch2(part + kWideRows * D + 2 * row);
+    floatx2 ml = {r.m, r.l[0]};
     floatx2 x[D / 4];
+    if (j == own) {
 #pragma unroll
-    for (int i = 0; i < D / 4; ++i) x[i] = fetch2(part + wave * (32 * D) + 128 * i + 2 * lane);
+      for (int i = 0; i < D / 4; ++i)
+        x[i] = floatx2{r.o[i / 8][2 * (i % 8)], r.o[i / 8][2 * (i % 8) + 1]};
+    } else {
+      const float *part = partial_of(p, 2 * (pc.first + j - 1) + (j == 0 ? 1 : 0), D);
+      ml = fetch2(part + kWideRows * D + 2 * row);
+#pragma unroll
+      for (int i = 0; i < D / 4; ++i) x[i] = fetch2(part + wave * (32 * D) + 128 * i + 2 * lane);
+    }
     const float top = fmaxf(m, ml[0]);
     const float a = m == -INFINITY ? 0.f : fast_exp2(m - top);
     const float b = ml[0] == -INFINITY ? 0.f : fast_exp2(ml[0] - top);
     m = top;
-    l = l * a + ml[1] * b;
+    l = fold(l, a, ml[1], b);
 #pragma unroll
     for (int i = 0; i < D / 4; ++i) {
-      o[i / 8][2 * (i % 8)] = o[i / 8][2 * (i % 8)] * a + x[i][0] * b;
-      o[i / 8][2 * (i % 8) + 1] = o[i / 8][2 * (i % 8) + 1] * a + x[i][1] * b;
+      o[i / 8][2 * (i % 8)] = fold(o[i / 8][2 * (i % 8)], a, x[i][0], b);
+      o[i / 8][2 * (i % 8) + 1] = fold(o[i / 8][2 * (i % 8) + 1], a, x[i][1], b);
     }
   }
   write_rows<T, D>(p, it, row, lane >> 5, o, l);
@@ -740,14 +861,21 @@ __device__ __forceinline__ void join_wide(const AttendPagedParams &p, const Item
 // k index 8 g + 4 part + e standing for key 16 part + 4 g + e of a 32-key step, which is how
 // the lane's own weights of two 16-key blocks lie; the lane gets dims 4 g + j.
 template <typename T, int D, int NQ>
-__device__ __forceinline__ void narrow_item(const AttendPagedParams &p, const Item &it,
-                                            unsigned ring, float *exchange, float *exchange_ml) {
+struct NarrowRows {
+  floatx4 o[NQ][D / 16];
+  float m[NQ], l[NQ];  // l: the lane's share of the row sum
+};
+
+// One pass over the wave's keys of a narrow item; CAREFUL as in wide_pass.
+template <typename T, int D, int NQ, bool CAREFUL>
+__device__ __forceinline__ void narrow_pass(ParamsRef p, const Item &it,
+                                            unsigned ring, NarrowRows<T, D, NQ> &r) {
   constexpr int kKeys = kNarrowKeys;
   constexpr int KB = kKeys / 16;
   constexpr int kTileBytes = kKeys * D * 2;
   constexpr int kLoads = kTileBytes / 1024;  // load instructions per tile
   const int lane = fresh_lane();  // per-lane offsets live in one kind of item only
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = it.wave;
   const int col = lane & 15, g = lane >> 4;
   const int rows = it.n * p.group;
   const unsigned k_tile = ring + wave * 2 * kTileBytes, v_tile = k_tile + kTileBytes;
@@ -786,8 +914,9 @@ __device__ __forceinline__ void narrow_item(const AttendPagedParams &p, const It
   for (int db = 0; db < D / 16; ++db)
     fv[db] = v_row * D + (((2 * db + ((col >> 1) & 1)) ^ group_v_swz<D>(v_row)) << 3) + 4 * (col & 1);
 
-  floatx4 o[NQ][D / 16];
-  float m[NQ], l[NQ];  // l: the lane's share of the row sum
+  auto &o = r.o;
+  auto &m = r.m;
+  auto &l = r.l;
 #pragma unroll
   for (int i = 0; i < NQ; ++i) {
     m[i] = -INFINITY;
@@ -811,7 +940,7 @@ __device__ __forceinline__ void narrow_item(const AttendPagedParams &p, const It
     for (int st = 0; st < D / 32; ++st)
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) k[st][kb] = read_frag<T>(k_tile, fk[st] + kb * 16 * D);
-  #pragma unroll
+#pragma unroll
     for (int st = 0; st < D / 32; ++st)
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
@@ -820,7 +949,8 @@ __device__ __forceinline__ void narrow_item(const AttendPagedParams &p, const It
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K is read before it is overwritten
     const WaveSlabs slabs = slabs_of<D>(p, it, ids, next);
     if (next < stop) issue(slabs, it.k, lo.k, k_tile);
-    if (absent != 0 || it.p0 < key0 + kKeys - 1 || key0 + kKeys > it.end) {
+    const bool masked = absent != 0 || it.p0 < key0 + kKeys - 1 || key0 + kKeys > it.end;
+    if (masked) {
 #pragma unroll
       for (int i = 0; i < NQ; ++i) {
         const int lim = min(pos[i], it.end - 1) - key0 - 4 * g;
@@ -865,49 +995,97 @@ __device__ __forceinline__ void narrow_item(const AttendPagedParams &p, const It
     if (next < stop) wait_loads<kLoads>();
     else wait_loads<0>();
     if (absent != 0 || key0 + kKeys > it.end) {
-      clear_v<D>(v_tile, kKeys, it.end - key0, absent, lane, kWave);
+      clear_v<D>(v_tile, kKeys, it.end - key0, absent, fresh_lane(), kWave);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
-    frag_t<T> v[D / 16][KB / 2];
+    if (CAREFUL && masked) {
 #pragma unroll
-    for (int db = 0; db < D / 16; ++db)
+      for (int i = 0; i < NQ; ++i)  // as accumulate_seen
+#pragma unroll 1
+        for (uint64_t todo = ~uint64_t{0}; todo != 0;) {
+          const unsigned tile = uniform_lds_u(v_tile);  // no address of this path is hoisted
+          const int at = __builtin_amdgcn_readlane(pos[i], __builtin_ctzll(todo));
+          todo &= ~__builtin_amdgcn_ballot_w64(pos[i] == at);
 #pragma unroll
-      for (int ks = 0; ks < KB / 2; ++ks)
-        v[db][ks] = read_v<T>(v_tile, fv[db] + 32 * ks * D, fv[db] + (32 * ks + 16) * D);
-  #pragma unroll
-    for (int db = 0; db < D / 16; ++db)
+          for (int db = 0; db < D / 16; ++db) {
+            floatx4 x = o[i][db];
 #pragma unroll
-      for (int ks = 0; ks < KB / 2; ++ks)
+            for (int ks = 0; ks < KB / 2; ++ks) {
+              const frag_t<T> v = keys_up_to<T, 16>(
+                  read_v<T>(tile, fv[db] + 32 * ks * D, fv[db] + (32 * ks + 16) * D),
+                  at - key0 - 4 * g - 32 * ks);
+              x = Frag<T>::mm16(v, hi[i][ks], x);
+              x = Frag<T>::mm16(v, low[i][ks], x);
+            }
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-          o[i][db] = Frag<T>::mm16(v[db][ks], hi[i][ks], o[i][db]);
-          o[i][db] = Frag<T>::mm16(v[db][ks], low[i][ks], o[i][db]);
+            for (int a = 0; a < 4; ++a) o[i][db][a] = pos[i] == at ? x[a] : o[i][db][a];
+            __builtin_amdgcn_sched_barrier(0);
+          }
         }
+    } else {
+      frag_t<T> v[D / 16][KB / 2];
+#pragma unroll
+      for (int db = 0; db < D / 16; ++db)
+#pragma unroll
+        for (int ks = 0; ks < KB / 2; ++ks)
+          v[db][ks] = read_v<T>(v_tile, fv[db] + 32 * ks * D, fv[db] + (32 * ks + 16) * D);
+#pragma unroll
+      for (int db = 0; db < D / 16; ++db)
+#pragma unroll
+        for (int ks = 0; ks < KB / 2; ++ks)
+#pragma unroll
+          for (int i = 0; i < NQ; ++i) {
+            o[i][db] = Frag<T>::mm16(v[db][ks], hi[i][ks], o[i][db]);
+            o[i][db] = Frag<T>::mm16(v[db][ks], low[i][ks], o[i][db]);
+          }
+    }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (next < stop) issue(slabs, it.v, lo.v, v_tile);
+  }
+}
+
+template <typename T, int D, int NQ>
+__device__ __forceinline__ void narrow_item(ParamsRef p, const Item &it,
+                                            unsigned ring, float *exchange, float *exchange_ml) {
+  const int rows = it.n * p.group, wave = it.wave;
+  NarrowRows<T, D, NQ> r;
+  narrow_pass<T, D, NQ, false>(p, it, ring, r);
+  // Rows of one token see the same keys: nothing that any of them should not see is left.
+  if (rows > p.group) {
+    float probe = 0.f;
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      probe += r.l[i];
+#pragma unroll
+      for (int db = 0; db < D / 16; ++db)
+#pragma unroll
+        for (int a = 0; a < 4; ++a) probe += r.o[i][db][a];
+    }
+    if (__builtin_amdgcn_ballot_w64(!is_finite(probe)) != 0)
+      narrow_pass<T, D, NQ, true>(p, it, ring, r);
   }
 
   // Join the four waves' states. Row r's dims lie in LDS as 16-byte pieces,
   // piece j at j ^ (r & 15).
+  const int lane = fresh_lane(), col = lane & 15, g = lane >> 4;
   block_barrier();  // every wave is done with its tiles
 #pragma unroll
   for (int i = 0; i < NQ; ++i) {
     const int row = 16 * i + col;
-    float sum = l[i] + __shfl_xor(l[i], 16);
-    sum += __shfl_xor(sum, 32);
+    const float sum = sum_lane_groups(r.l[i]);
     if (row < rows) {
       float *x = exchange + (wave * kNarrowRows + row) * D;
 #pragma unroll
       for (int db = 0; db < D / 16; ++db)
-        *reinterpret_cast<floatx4 *>(x + 4 * ((4 * db + g) ^ col)) = o[i][db];
+        *reinterpret_cast<floatx4 *>(x + 4 * ((4 * db + g) ^ col)) = r.o[i][db];
       if (g == 0) {
-        exchange_ml[2 * (wave * kNarrowRows + row)] = m[i];
+        exchange_ml[2 * (wave * kNarrowRows + row)] = r.m[i];
         exchange_ml[2 * (wave * kNarrowRows + row) + 1] = sum;
       }
     }
   }
   block_barrier();
-  for (int i = threadIdx.x; i < rows * (D / 2); i += kThreads) {
+  for (int i = 64 * wave + lane; i < rows * (D / 2); i += kThreads) {
     const int at = i / (D / 2), pair = i % (D / 2);  // two dims per thread
     float m = -INFINITY, l = 0.f;
     float w[kWaves];
@@ -940,12 +1118,13 @@ __device__ __forceinline__ void narrow_item(const AttendPagedParams &p, const It
 // Joins a narrow item's pieces, first to last, and writes its rows. Eight pieces' loads
 // are in flight at a time.
 template <typename T, int D>
-__device__ __forceinline__ void join_narrow(const AttendPagedParams &p, const Item &it,
+__device__ __forceinline__ void join_narrow(ParamsRef p, const Item &it,
                                             const Pieces &pc) {
   constexpr int kDeep = 8;
   typedef T t2 __attribute__((ext_vector_type(2)));
   const int n = it.n * p.group * (D / 2);
-  for (int i = threadIdx.x; i < n; i += kThreads) {
+  const int thread = 64 * it.wave + fresh_lane();
+  for (int i = thread; i < n; i += kThreads) {
     const int row = i / (D / 2), at = 2 * (i % (D / 2));
     float m = -INFINITY, l = 0.f;
     floatx2 o = {0.f, 0.f};
@@ -983,11 +1162,13 @@ __device__ __forceinline__ void join_narrow(const AttendPagedParams &p, const It
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, Geo<D>::kBlocks) void attend_paged_kernel(const AttendPagedParams p) {
+__global__ __launch_bounds__(kThreads, Geo<D>::kBlocks) void attend_paged_kernel(const AttendPagedParams) {
   __shared__ __align__(1024) unsigned char ring_mem[Geo<D>::kRingBytes];
   __shared__ __align__(16) float ml_mem[2 * kWaves * kNarrowRows];
-  __shared__ int arrived;
+  __shared__ int arrived, votes[kWaves];
 
+  const ParamsPtr params = (ParamsPtr)__builtin_amdgcn_kernarg_segment_ptr();
+  ParamsRef p = *params;
   // One word of each 64-byte line of the arguments, read together: the lines' misses
   // (their first use in a launch) overlap instead of following one another.
   {
@@ -997,18 +1178,18 @@ __global__ __launch_bounds__(kThreads, Geo<D>::kBlocks) void attend_paged_kernel
     for (unsigned i = 0; i < sizeof(AttendPagedParams); i += 64) touched ^= args[i / 4];
     asm volatile("" ::"s"(touched));
   }
-  const int tid = static_cast<int>(threadIdx.x);
-  const int lane = tid & 63;
+  const int lane = static_cast<int>(threadIdx.x) & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int n_blocks = static_cast<int>(gridDim.x);
   const uniform_ints bounds = uniform_at(p.cu_tokens), lens = uniform_at(p.seq_lens);
   // Packed rows that belong to no sequence: [0, head) and [tail, tokens).
   const int head = min(max(bounds[0], 0), p.tokens);
-  const int tail = min(max(bounds[p.batch], 0), p.tokens);
+  const int last_bound = min(max(bounds[p.batch], 0), p.tokens);
 
   // Every wave sums the sequences' weights (lane l takes `per` of them) and finds its
   // block's two borders: no exchange between waves, and scalar code from there on.
   const int per = (p.batch + kWave - 1) / kWave;
-  int mine = 0, my_items = 0;
+  int mine = 0, my_items = 0, my_tokens = 0;
   Seq s = {0, 0, 0};
   for (int i = 0; i < per; ++i) {
     const int b = lane * per + i;
@@ -1017,8 +1198,13 @@ __global__ __launch_bounds__(kThreads, Geo<D>::kBlocks) void attend_paged_kernel
     const Tiles t = tiles_of<false>(p, s.n);
     mine += keys_before(p, s, t, t.count) * p.kv_heads;
     my_items += t.count * p.kv_heads;
+    my_tokens = min(my_tokens + s.n, p.tokens + 1);
   }
   const int keys_upto = wave_prefix(mine), items_upto = wave_prefix(my_items);
+  // Bounds that go up and down can claim more rows than there are, beyond what the weights'
+  // 30 bits were chosen for: such a batch has no sequences, and its outputs are zero.
+  const bool sound = __builtin_amdgcn_readlane(wave_prefix(my_tokens), kWave - 1) <= p.tokens;
+  const int tail = sound ? last_bound : 0;
   const int all_keys = __builtin_amdgcn_readlane(keys_upto, kWave - 1);
   const int all_items = __builtin_amdgcn_readlane(items_upto, kWave - 1);
   const int few = 1 + (kFewItemKeys >> p.unit);
@@ -1050,7 +1236,7 @@ __global__ __launch_bounds__(kThreads, Geo<D>::kBlocks) void attend_paged_kernel
     border.s.t0 = __shfl(s.t0, owner & 63);
     border.s.n = __shfl(s.n, owner & 63);
     border.s.p0 = __shfl(s.p0, owner & 63);
-  } else if (owner < kWave) {
+  } else if (sound && owner < kWave) {
     for (;; ++border.b) {  // the owner's sequences
       border.s = load_seq(p, p.cu_tokens, p.seq_lens, border.b);
       const Tiles t = tiles_of<false>(p, border.s.n);
@@ -1059,7 +1245,7 @@ __global__ __launch_bounds__(kThreads, Geo<D>::kBlocks) void attend_paged_kernel
       border.from += weight;
     }
   }
-  if (owner < kWave) place_border(p, tiles_of<false>(p, border.s.n), item, at, border);
+  if (sound && owner < kWave) place_border(p, tiles_of<false>(p, border.s.n), item, at, border);
   else border.b = p.batch;
   struct { int b, kvh, tile, kt; } end;
   int b = __builtin_amdgcn_readlane(border.b, 0), kvh = __builtin_amdgcn_readlane(border.kvh, 0);
@@ -1075,7 +1261,7 @@ __global__ __launch_bounds__(kThreads, Geo<D>::kBlocks) void attend_paged_kernel
 
   const unsigned ring = lds_addr(ring_mem);
   Tiles t = tiles_of<true>(p, s.n);
-  while (b < p.batch) {
+  while (sound && b < p.batch) {
     if (tile >= t.count) {  // next K/V head or sequence
       tile = 0;
       kt = 0;
@@ -1100,6 +1286,7 @@ __global__ __launch_bounds__(kThreads, Geo<D>::kBlocks) void attend_paged_kernel
     it.n = min(t.tokens, s.n - tile * t.tokens);
     it.p0 = s.p0 + tile * t.tokens;
     it.kvh = kvh;
+    it.wave = wave;
     const uint64_t head_at = static_cast<uint64_t>(kvh) * p.head_bytes;
     it.k = static_cast<const char *>(p.k_pages) + head_at;
     it.v = static_cast<const char *>(p.v_pages) + head_at;
@@ -1109,35 +1296,37 @@ __global__ __launch_bounds__(kThreads, Geo<D>::kBlocks) void attend_paged_kernel
                        !(last && tiles == 0);
     if (whole || it.kt1 > it.kt0) {
       it.slot = whole ? -1 : 2 * w + (it.kt0 == 0 ? 1 : 0);
-      if (it.n * p.group <= 16)
-        narrow_item<T, D, 1>(p, it, ring, reinterpret_cast<float *>(ring_mem), ml_mem);
-      else if (it.n * p.group <= kNarrowRows)
-        narrow_item<T, D, 2>(p, it, ring, reinterpret_cast<float *>(ring_mem), ml_mem);
-      else
-        wide_item<T, D>(p, it, ring);
-    }
-    if (!whole && it.kt1 > it.kt0) {
-      const int x0 = from + kvh * weight_before(p, s, t, item, t.count) + weight_before(p, s, t, item, tile);
-      const int x1 = x0 + weight_before(p, s, t, item, tile + 1) - weight_before(p, s, t, item, tile);
-      const Pieces pc = pieces_of(p, t, item, x0, x1, tiles, share);
-      // The partial is stored before it is counted; the block that counts last sets the
-      // counter back to zero for the next call.
-      wait_loads<0>();
-      __syncthreads();
-      if (tid == 0) {
-        unsigned *counter = p.counters + pc.first;
-        const unsigned n = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED,
-                                                  __HIP_MEMORY_SCOPE_AGENT);
-        arrived = static_cast<int>(n) + 1;
-        if (arrived == pc.count)
-          __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      Pieces pc;
+      // A partial is stored before it is counted; the block that counts last sets the
+      // counter back to zero for the next call, and joins the pieces.
+      auto counts_last = [&] {
+        const int x0 = from + kvh * weight_before(p, s, t, item, t.count) +
+                       weight_before(p, s, t, item, tile);
+        const int x1 = x0 + weight_before(p, s, t, item, tile + 1) - weight_before(p, s, t, item, tile);
+        pc = pieces_of(p, t, item, x0, x1, tiles, share);
+        wait_loads<0>();
+        __syncthreads();
+        if (wave == 0 && fresh_lane() == 0) {
+          unsigned *counter = p.counters + pc.first;
+          arrived = 1 + static_cast<int>(__hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED,
+                                                                __HIP_MEMORY_SCOPE_AGENT));
+          if (arrived == pc.count)
+            __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        return arrived == pc.count;
+      };
+      if (it.n * p.group <= kNarrowRows) {
+        float *exchange = reinterpret_cast<float *>(ring_mem);
+        if (it.n * p.group <= 16) narrow_item<T, D, 1>(anew(params), it, ring, exchange, ml_mem);
+        else narrow_item<T, D, 2>(anew(params), it, ring, exchange, ml_mem);
+        if (!whole && counts_last()) join_narrow<T, D>(anew(params), it, pc);
+      } else {
+        Rows<T, D> r;
+        wide_item<T, D>(anew(params), it, ring, votes, r);
+        if (!whole && counts_last()) join_wide<T, D>(anew(params), it, pc, w - pc.first + 1, r);
       }
-      __syncthreads();
-      if (arrived == pc.count) {
-        if (it.n * p.group <= kNarrowRows) join_narrow<T, D>(p, it, pc);
-        else join_wide<T, D>(p, it, pc);
-      }
-      __syncthreads();
+      if (!whole) __syncthreads();  // `arrived` may be written again
     }
     if (last) break;
     ++tile;
@@ -1145,10 +1334,10 @@ __global__ __launch_bounds__(kThreads, Geo<D>::kBlocks) void attend_paged_kernel
   }
 
   // Outputs of packed rows that belong to no sequence are zero.
-  if (head + p.tokens - tail <= 0) return;
+  if (sound && head + p.tokens - tail <= 0) return;
   const int64_t per_row = static_cast<int64_t>(p.heads) * (D / 8);
   const int64_t outside = (static_cast<int64_t>(head) + p.tokens - tail) * per_row;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + tid; i < outside;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + 64 * wave + fresh_lane(); i < outside;
        i += static_cast<int64_t>(n_blocks) * kThreads) {
     const int64_t at = i < head * per_row ? i : i + (static_cast<int64_t>(tail) - head) * per_row;
     const uint4 zero = {0, 0, 0, 0};

@@ -90,6 +90,51 @@ def test_rows_that_hold_no_key_do_not_matter(name, junk):
     assert torch.equal(_attend(s, 0.125), want)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,kv_heads", [(6, 2), (14, 1)])
+@pytest.mark.parametrize("where", [(1, 2, 3), (0, 5, 40), (130, 131, 149)])
+def test_later_tokens_that_are_not_finite_do_not_matter(dtype, dim, heads, kv_heads, where):
+    """A token's NaN or infinity reaches the queries at and after it, and no other:
+    not through a weight of zero (0 * inf) of a query before it."""
+    s = ref.batch([(9, 150), (33, 4), (60, 8)], kv_heads, heads, dim, 16, dtype, 40)
+    want = _attend(s, 0.125).cpu()
+    at = [w for w in where], [33 + 1, 33 + 2], [60 + 3]
+    for b, tokens in enumerate(at):
+        for i, token in enumerate(tokens):
+            pos = token + (9 if b == 0 else 0)
+            page = s["page_table"][b, pos // 16]
+            s["v_pages"][page, :, pos % 16, i::5] = [float("inf"), float("nan"), -float("inf")][i % 3]
+            s["k_pages"][page, :, pos % 16, 0] = float("nan")
+    got = _attend(s, 0.125).cpu()
+    bounds = s["cu_tokens"].tolist()
+    for b, first in enumerate([min(where), 1, 3]):
+        assert torch.equal(got[bounds[b]:bounds[b] + first], want[bounds[b]:bounds[b] + first])
+        assert not torch.isfinite(got[bounds[b] + first:bounds[b + 1]]).any()
+
+
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
+@pytest.mark.parametrize("name", ["drafts", "chunks"])
+def test_infinite_values_reach_only_their_dims(value, name):
+    """With finite keys, a value dim that is not finite leaves that dim not finite for
+    the queries that see it, and changes no other. (Items of few rows, also the last
+    ones of a chunk, split each weight into hi + lo with |lo| <= hi / 2048 of either
+    sign, so an infinity may come out as inf hi + inf lo = NaN.)"""
+    s = ref.batch(SEQUENCES[name], 2, 6, 64, 16, torch.float16, 41)
+    want = _attend(s, 0.125).cpu()
+    bounds, lens = s["cu_tokens"].tolist(), s["seq_lens"].tolist()
+    for b, n in enumerate(lens):
+        pos = n - 2
+        s["v_pages"][s["page_table"][b, pos // 16], :, pos % 16, 7] = value
+    got = _attend(s, 0.125).cpu()
+    for b in range(len(lens)):
+        before, after = slice(bounds[b], bounds[b + 1] - 2), slice(bounds[b + 1] - 2, bounds[b + 1])
+        assert torch.equal(got[before], want[before])
+        rest = [d for d in range(64) if d != 7]
+        assert torch.equal(got[after][..., rest], want[after][..., rest])
+        assert not torch.isfinite(got[after][..., 7]).any()
+
+
 @pytest.mark.parametrize("page", [16, 64])
 @pytest.mark.parametrize("name", ["tokens", "mixed", "chunks"])
 def test_page_ids_outside_the_pool_have_no_keys(page, name):
@@ -124,6 +169,19 @@ def test_token_bounds_that_do_not_fit_the_tensor():
     s["cu_tokens"] = torch.tensor([4, 9, 9], dtype=torch.int32)
     got = _attend(s, 0.125).cpu()
     assert (got[:4] == 0).all() and (got[9:] == 0).all() and (got[4:9] != 0).any()
+
+
+@pytest.mark.parametrize("repeats", [3, 200])
+def test_bounds_that_fall_have_no_sequences(repeats):
+    """Bounds that go up and down claim more rows than there are: the outputs are
+    zero, and the next call is as if nothing had been."""
+    s = ref.batch([(40, 20)] * repeats, 1, 4, 64, 16, torch.float16, 42)
+    want = _attend(s, 0.125)
+    good = s["cu_tokens"].clone()
+    s["cu_tokens"][0::2], s["cu_tokens"][1::2] = 0, s["q"].shape[0]
+    assert (_attend(s, 0.125) == 0).all()
+    s["cu_tokens"] = good
+    assert torch.equal(_attend(s, 0.125), want)
 
 
 def test_attend_takes_slices_of_a_projection():
