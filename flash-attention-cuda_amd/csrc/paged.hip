@@ -15,15 +15,17 @@
 //            for the whole group. A sequence of at most 32 rows is one "narrow"
 //            item; others are tiles of up to 128 rows of whole tokens.
 //   share  = the items laid end to end, weighted by the keys they see, are cut
-//            into equal shares, one per block (two blocks per CU): ragged
-//            lengths and few sequences fill the chip alike, without a host
-//            that knows the lengths. Each block finds its own share from
-//            seq_lens and cu_tokens.
+//            into equal shares, one per block (two or three blocks per CU):
+//            ragged lengths and few sequences fill the chip alike, without a
+//            host that knows the lengths. Each wave finds its block's share
+//            from seq_lens and cu_tokens (1 us: kernel arguments, lengths, a
+//            sum over the lanes, 32-bit arithmetic).
 //   merge  = an item that a share's border cuts leaves one fp32 partial (O, m,
 //            l) per share in the workspace; the block that finishes last joins
-//            them in the order of the shares, so results do not depend on timing.
+//            them in the order of the shares, so results do not depend on timing
+//            (a second launch for it took 2.6 to 18.7 us).
 //
-// Block: 256 threads, 4 waves, two blocks per CU.
+// Block: 256 threads, 4 waves.
 //   wide item: wave w owns query rows [32 w, +32); the waves share 64-key K and V
 //     tiles in an LDS ring filled by direct global->LDS loads.
 //   narrow item: the waves take key tiles in turn, each with K and V tiles of its
@@ -33,13 +35,26 @@
 //
 // Roundings to 16 bits. P is rounded once on wide items (the row sum is taken of
 // the rounded weights, so a row that one key carries is exact) and split into two
-// parts on narrow ones, where memory is what bounds the loop.
+// parts on narrow ones, where memory is what bounds the loop: against 64 bits (relative
+// 2-norm, N(0,1)) fp16 outputs of wide items are 2.6e-4 to 2.9e-4 off, of narrow ones
+// 2.0e-4 (the output's own rounding); bf16 2.3e-3 and 1.7e-3.
+//
+// Measured (us per call among others; B sequences, H / H_kv heads, D head_dim):
+//   B1 H12 D64, 512 keys, one token             7.2   chain of a block's loads (6 us of GPU)
+//   B32 H14/2 D64, 4096 keys ragged, one token 14.1   2.5 TB/s: share 2 us, ~4 rounds of
+//                                                     loads, publish and join 2 us
+//   B8 H32/8 D128 bf16, 8191 ragged, one token 31.5   4.8 TB/s of K and V: HBM
+//   B1 H14 D64, prompt of 4096                 53.1   566 TFLOP/s; MFMA 32 %, VALU 50 % busy
+//   B24 H28/4 D128, 3 chunks to 777 + tokens   48.8   2.6 TB/s and 330 TFLOP/s
+//   B4 H32/8 D128 bf16, chunks to 2048 on 6144  482   936 TFLOP/s; MFMA 48 %, VALU 35 % busy:
+//                                                     the two hardly run at once
 //
 // Memory safety. Lengths, bounds and page ids are device data, which the host
 // cannot check: token ranges are clamped to the packed tensors, key ranges to the
 // page table's width, and a page id outside the pool is replaced by page 0 for
 // the address and its keys are masked out. V rows past a sequence's end
-// are cleared in LDS before they meet a weight of zero (0 * NaN).
+// are cleared in LDS before they meet a weight of zero (0 * NaN); what a query may not
+// see for its position does not reach it either (wide_pass).
 
 #include "mfma_tile.h"
 
@@ -52,14 +67,28 @@ constexpr int kTileKeys = 64;     // keys per tile of a wide item, and the unit 
 constexpr int kWideRows = 128;    // query rows of a wide item
 constexpr int kNarrowRows = 32;   // most query rows of a narrow item
 constexpr int kNarrowKeys = 32;   // keys of a narrow item's tile, of which each wave has its own
-constexpr int kItemKeys = 320;    // an item's fixed cost, in keys, when there are many
-constexpr int kFewItemKeys = 512; // and when blocks are to spare: no block takes two items
-constexpr int kMinShareKeys = 512;  // least weight of a share
-constexpr int kWideStep = 2;      // borders inside wide items lie at multiples of this many tiles
-constexpr int kWholeSteps = 4;    // items of at most this many steps are never cut
+
+// Weights of the shares, measured over the cases above and 16 random batches:
+// An item's fixed cost (start, partial, join) in keys: 320 where there are many (192: B8
+// H32/8 D128 33.5 us for 32.0, mixed 54.0 for 52.5; 128: mixed 61; 384 as 320), and
+// 512, the least share, where there are blocks to spare, so that no block takes two items
+// (13 prompts of ~138 tokens 21.4 -> 12.9 us, 24 short sequences 11.4 -> 7.7).
+constexpr int kItemKeys = 320;
+constexpr int kFewItemKeys = 512;
+// Least weight of a share: 512 keys (256: two sequences of 8k keys 19.0 us for 16.9;
+// 640 and more: 32 ragged sequences 15.9 for 15.0).
+constexpr int kMinShareKeys = 512;
+// Borders inside wide items lie at multiples of this many tiles (1 alike; 4: prompt 62 us
+// for 57), inside narrow ones at a round of the block's waves; items of at most kWholeSteps
+// such steps are never cut, since a cut costs about as much as two of them.
+constexpr int kWideStep = 2;
+constexpr int kWholeSteps = 4;
 
 // Blocks per CU and LDS for tiles per block, by head size. A head_dim 64 wave fits 168
-// VGPRs, so three blocks share a CU.
+// VGPRs, so three blocks share a CU (two: prompt 57.3 us for 55.4, 20 sequences with 4
+// chunks 48.2 for 45.4). At head_dim 128, one block of 8 waves with 256-row items instead of
+// two of 4 halves the tile loads (long chunks 477 us for 496, long tokens 29.8 for 31.5) but
+// leaves shorter chunks worse dealt (mixed 70 for 50).
 template <int D>
 struct Geo;
 template <>
@@ -76,7 +105,6 @@ struct Frag;
 template <>
 struct Frag<_Float16> {
   typedef half8 type;
-  typedef half2 pair;
   static __device__ __forceinline__ floatx16 mm(type a, type b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
@@ -87,7 +115,6 @@ struct Frag<_Float16> {
 template <>
 struct Frag<__bf16> {
   typedef __bf16 type __attribute__((ext_vector_type(8)));
-  typedef __bf16 pair __attribute__((ext_vector_type(2)));
   static __device__ __forceinline__ floatx16 mm(type a, type b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -303,7 +330,7 @@ struct Item {
   int t0, n, p0;     // packed tokens and the first one's position
   int kvh;
   int kt0, kt1;      // key tiles of this share
-  int end;           // keys the item sees (the last token's)
+  int end, last;     // keys the item sees (the last token's), and the last one (0 without any)
   int slot;          // partial slot, -1: the whole item
   int wave;          // the calling wave's index in its block
   uniform_ints table;
@@ -337,8 +364,9 @@ __device__ __forceinline__ frag_t<T> read_frag(unsigned tile, int off) {
   return *reinterpret_cast<lds_frag *>(static_cast<uintptr_t>(tile + 2u * off));
 }
 
-// All of a tile's K operands, read before the first product: a product that waits for its
-// own read costs the LDS latency each time (at XX).
+// The reads of a tile's K operands run ahead of the products, as the compiler schedules them:
+// with addresses that it could not move a read past, each product waited for its own
+// read (long chunks of head_dim 128 515 us for 482).
 template <typename T, int D, int KB>
 __device__ __forceinline__ void scores(unsigned tile, const FragOffsetsD<D> &fo,
                                        const Rows<T, D> &r, floatx16 (&s)[KB]) {
@@ -357,7 +385,8 @@ __device__ __forceinline__ void scores(unsigned tile, const FragOffsetsD<D> &fo,
     for (int kb = 0; kb < KB; ++kb) s[kb] = Frag<T>::mm(k[i][kb], r.q[i], s[kb]);
 }
 
-// All of a tile's V^T operands; they land under the softmax.
+// All of a tile's V^T operands. (Read before the softmax, to land under it: no faster, with
+// every register taken.)
 template <typename T, int D, int KB>
 struct ValueFrags {
   frag_t<T> f[D / 32][2 * KB];
@@ -386,9 +415,9 @@ __device__ __forceinline__ void hide(floatx16 (&s)[KB], int lim, unsigned absent
     }
 }
 
-// Weights of the tile as P^T fragments. The bound m
-// moves only when a row's scores pass it by more than 2^8 (weights up to 2^8 are
-// harmless in either type): O is rescaled a few times per item instead of per tile.
+// Weights of the tile as P^T fragments. The bound m moves only when a row's scores pass it by
+// more than 2^8 (weights up to 2^8 are harmless in either type): O is rescaled a few times
+// per item instead of per tile.
 template <typename T, int D, int KB>
 __device__ __forceinline__ void weigh(floatx16 (&s)[KB], float c, Rows<T, D> &r,
                                       frag_t<T> (&w)[2 * KB]) {
@@ -498,7 +527,8 @@ __device__ __forceinline__ void accumulate_seen(unsigned tile, const FragOffsets
 // ---- pages --------------------------------------------------------------------------
 
 // Page ids of the N 16-key slabs from `key` on: N scalar loads, in flight together. Keys
-// past the end lie on no page of their own: the last key's page stands in.
+// past the end lie on no page of their own: the last key's page stands in (the first page of
+// an item without keys, which loads nothing).
 template <int N>
 struct PageIds {
   int id[N];
@@ -508,7 +538,8 @@ __device__ __forceinline__ PageIds<N> page_ids(ParamsRef p, const Item &it,
                                                int key) {
   PageIds<N> r;
 #pragma unroll
-  for (int i = 0; i < N; ++i) r.id[i] = it.table[min(key + 16 * i, it.end - 1) >> p.page_shift];
+  for (int i = 0; i < N; ++i)
+    r.id[i] = it.table[min(key + 16 * i, it.last) >> p.page_shift];
   return r;
 }
 __device__ __forceinline__ bool is_absent(ParamsRef p, int id) {
@@ -854,8 +885,8 @@ __device__ __forceinline__ void join_wide(ParamsRef p, const Item &it,
 }
 
 // Narrow items run on v_mfma_f32_16x16x32, with NQ groups of 16 query rows: with the
-// 32-row products a group of 7 query heads paid for 32 rows of softmax, 2600 cycles per
-// 64-key tile of head_dim 64 against XX.
+// 32-row products a group of 7 query heads paid for 32 rows of softmax (32 ragged sequences
+// of 14/2 heads 16.3 us for 14.5).
 // Lane l: query l % 16 of a group, g = l / 16. S^T of 16 keys: A = K rows (k-step s, lane g:
 // dims [32 s + 8 g, +8)), B = Q^T alike; the lane gets keys 4 g + j. O^T of 16 dims: A = V^T,
 // k index 8 g + 4 part + e standing for key 16 part + 4 g + e of a 32-key step, which is how
@@ -1116,7 +1147,7 @@ __device__ __forceinline__ void narrow_item(ParamsRef p, const Item &it,
 }
 
 // Joins a narrow item's pieces, first to last, and writes its rows. Eight pieces' loads
-// are in flight at a time.
+// are in flight at a time (16: 15.7 us for 15.1 where items have about 8; 4 alike).
 template <typename T, int D>
 __device__ __forceinline__ void join_narrow(ParamsRef p, const Item &it,
                                             const Pieces &pc) {
@@ -1208,8 +1239,9 @@ __global__ __launch_bounds__(kThreads, Geo<D>::kBlocks) void attend_paged_kernel
   const int all_keys = __builtin_amdgcn_readlane(keys_upto, kWave - 1);
   const int all_items = __builtin_amdgcn_readlane(items_upto, kWave - 1);
   const int few = 1 + (kFewItemKeys >> p.unit);
-  const int item = all_items <= n_blocks && all_keys + all_items * few <= n_blocks * few
-                       ? few : 1 + (kItemKeys >> p.unit);
+  const int item = __builtin_amdgcn_readfirstlane(
+      all_items <= n_blocks && all_keys + all_items * few <= n_blocks * few
+          ? few : 1 + (kItemKeys >> p.unit));
   const int total = all_keys + all_items * item;
   mine += my_items * item;
   const int upto = keys_upto + items_upto * item;
@@ -1260,6 +1292,7 @@ __global__ __launch_bounds__(kThreads, Geo<D>::kBlocks) void attend_paged_kernel
   end.kt = __builtin_amdgcn_readlane(border.kt, 1);
 
   const unsigned ring = lds_addr(ring_mem);
+  const int all_weight = __builtin_amdgcn_readfirstlane(total);
   Tiles t = tiles_of<true>(p, s.n);
   while (sound && b < p.batch) {
     if (tile >= t.count) {  // next K/V head or sequence
@@ -1268,7 +1301,8 @@ __global__ __launch_bounds__(kThreads, Geo<D>::kBlocks) void attend_paged_kernel
       if (t.count == 0 || ++kvh >= p.kv_heads) {
         from += weight_before(p, s, t, item, t.count) * p.kv_heads;
         kvh = 0;
-        ++b;
+        // Nothing but empty sequences follows the last weight.
+        b = __builtin_amdgcn_readfirstlane(from) >= all_weight ? p.batch : b + 1;
         if (b >= p.batch) break;
         s = load_seq(p, bounds, lens, b);
         t = tiles_of<true>(p, s.n);
@@ -1279,6 +1313,7 @@ __global__ __launch_bounds__(kThreads, Geo<D>::kBlocks) void attend_paged_kernel
     const bool last = b == end.b && kvh == end.kvh && tile == end.tile;
     Item it;
     it.end = key_end(p, s, t, tile);
+    it.last = __builtin_amdgcn_readfirstlane(max(it.end - 1, 0));
     const int tiles = key_tiles(it.end);
     it.kt0 = kt;
     it.kt1 = last ? min(end.kt, tiles) : tiles;
@@ -1391,8 +1426,11 @@ int launch_attend_paged(AttendPagedParams p, bool bf16, int head_dim, float scal
   p.narrow_step = kWaves * kNarrowKeys / kTileKeys;
   p.wide_inv = 1.0f / static_cast<float>(p.wide_tokens);
   p.group_inv = (65536 + p.group - 1) / p.group;
-  // Weight of any batch of this many tokens and sequences.
-  const double tiles = static_cast<double>(p.tokens) / p.wide_tokens + p.batch;
+  // Weight of any batch of this many tokens and sequences (those without tokens have none).
+  const double tiles = static_cast<double>(p.tokens) / p.wide_tokens + min(p.batch, p.tokens);
+  if (tiles * p.kv_heads > 5e8)
+    return set_error(FA_ERR_INVALID_ARGUMENT, "too many query tiles: %d tokens, H=%d H_kv=%d",
+                     p.tokens, p.heads, p.kv_heads);
   const double most =
       tiles * p.kv_heads * (2.0 + p.capacity + kItemKeys + p.tokens + 2.0 * p.wide_tokens);
   p.unit = 0;

@@ -514,9 +514,10 @@ int check_paged(const fa_paged *c, int *page_shift) {
     return set_error(FA_ERR_INVALID_ARGUMENT, "max_pages * page_size must be at most %d, got %lld",
                      kMaxCacheRows, static_cast<long long>(c->max_pages) * c->page_size);
   // Threads of the append's grid, and row indices of the attention, stay in int.
-  if (c->tokens > (1 << 24) || c->batch > (1 << 24))
+  if (c->tokens > (1 << 24) || c->batch > (1 << 16))
     return set_error(FA_ERR_INVALID_ARGUMENT,
-                     "at most 2^24 packed tokens and sequences, got %d and %d", c->tokens, c->batch);
+                     "at most 2^24 packed tokens and 2^16 sequences, got %d and %d", c->tokens,
+                     c->batch);
   if (c->kv_heads > 8192)
     return set_error(FA_ERR_INVALID_ARGUMENT, "at most 8192 K/V heads, got %d", c->kv_heads);
   *page_shift = __builtin_ctz(static_cast<unsigned>(c->page_size));

@@ -284,8 +284,9 @@ int fa_rope(const void *x, void *out, const int32_t *positions, const double *in
  * page_table, seq_lens and cu_tokens (batch + 1 entries, the first 0, rising) are
  * int32 in device memory and never read on the host. What they hold cannot lead a
  * kernel out of the tensors: a position outside [0, max_pages * page_size) or a
- * page id outside [0, num_pages) has no key; packed rows from cu_tokens[batch] on
- * belong to no sequence. */
+ * page id outside [0, num_pages) has no key; packed rows before cu_tokens[0] and from
+ * cu_tokens[batch] on belong to no sequence. At most 2^24 packed rows and 2^16
+ * sequences; max_pages * page_size at most 2^27. */
 typedef struct fa_paged {
   void *k_pages, *v_pages;
   const int32_t *page_table, *seq_lens, *cu_tokens;
@@ -305,7 +306,8 @@ typedef struct fa_rows {
  * fa_rope), and q, H = `heads` query heads, is turned into q_out, contiguous
  * [tokens, H, head_dim] (rows that belong to no sequence become zero); with
  * rotary_dim 0, q, q_out and inv_freq are not used. Lengths are not changed: the
- * call can be repeated. No two tokens may have the same place. */
+ * call can be repeated. No two tokens may have the same place, and q_out overlaps
+ * no input. */
 int fa_append_paged(const fa_paged *cache, const fa_rows *k, const fa_rows *v, const fa_rows *q,
                     void *q_out, int heads, const double *inv_freq, int rotary_dim,
                     int interleaved, float factor, void *stream);
@@ -317,8 +319,13 @@ size_t fa_attend_paged_workspace_bytes(int tokens, int heads, int kv_heads, int 
 /* Causal attention of the new tokens' queries over the cache, their own keys
  * (written before) among it: o[t, h] = softmax over keys 0..position(t) of
  * scale * q[t, h] . k, times v, with K/V head h / (H / H_kv). out is contiguous
- * [tokens, H, head_dim]; a row without a key, and one that belongs to no sequence,
- * is zero. At most 128 query heads per K/V head. */
+ * [tokens, H, head_dim] and overlaps no input; a row without a key, and one that
+ * belongs to no sequence, is zero; so is every row if cu_tokens rises and falls so
+ * that the sequences claim more rows than there are. What a query does not see does not
+ * reach it, infinities and NaN included. At most 128 query heads per K/V head.
+ * Workspace and streams follow the rules of the split-K decode: the workspace stays
+ * untouched until the launch completes, calls on one stream are ordered, replays of
+ * one graph must not overlap. */
 int fa_attend_paged(const fa_paged *cache, const fa_rows *q, void *out, int heads, float scale,
                     void *workspace, size_t workspace_bytes, void *stream);
 

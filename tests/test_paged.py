@@ -392,6 +392,26 @@ def test_a_captured_step_replays(dtype):
             assert torch.equal(a, b)
 
 
+def test_many_empty_sequences_and_more_streams_than_counters():
+    """Thousands of sequences without tokens around a few with them; the calls run
+    on fresh captures until the library has no arrival counters left for one, and
+    keep their results."""
+    sequences = [(0, 0)] * 3000 + [(2900, 3), (40, 1)] + [(0, 0)] * 2000 + [(700, 40)] + [(0, 0)] * 999
+    s = ref.batch(sequences, 1, 4, 64, 16, torch.float16, 21)
+    want = _attend(s, 0.125)
+    check, bound = ref.attend(s["q"], *(s[name] for name in CACHE), 0.125)
+    assert ((want.cpu().double() - check).abs() <= bound).all()
+    args = s["q"].cuda(), *(s[name].cuda() for name in CACHE), 0.125
+    for _ in range(70):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = flashattn_cuda.attend_paged(*args)
+        graph.replay()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
 def test_two_streams_at_once():
     batches = [ref.batch([(3001, 40), (10, 1)], 2, 4, 64, 16, torch.float16, 20 + i)
                for i in range(2)]

@@ -48,7 +48,7 @@ BAD_CACHE = [
     (dict(head_dim=96), "head_dim"), (dict(page_size=8), "power of two"),
     (dict(page_size=48), "power of two"), (dict(page_size=2048), "power of two"),
     (dict(page_size=1024, max_pages=2 ** 20), "max_pages * page_size"),
-    (dict(tokens=2 ** 24 + 1), "packed tokens"), (dict(kv_heads=8193), "K/V heads"),
+    (dict(tokens=2 ** 24 + 1), "packed tokens"), (dict(batch=2 ** 16 + 1), "2^16 sequences"), (dict(kv_heads=8193), "K/V heads"),
 ]
 
 
