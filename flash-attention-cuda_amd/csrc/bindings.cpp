@@ -31,6 +31,7 @@
 #include <vector>
 
 #include "flashattn_hip.h"
+#include "flashattn_hip/paged.h"
 
 namespace {
 

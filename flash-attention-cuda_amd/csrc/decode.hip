@@ -240,9 +240,11 @@ __device__ __forceinline__ void merge_state(float &m, float &l, float acc[8],
 // so a finished call leaves every counter at zero. The counters are zero when
 // the code object loads and are split into slots, one per (device, stream)
 // in use, so calls that may overlap in time (other streams) never share one.
+// attend_paged has slots of its own, so its streams and captures take none of
+// those that decode and prefill find here.
 constexpr int kCounterSlots = 64;
 constexpr int kCountersPerSlot = static_cast<int>(kMergeCountersPerSlot);
-__device__ unsigned g_merge_counters[kCounterSlots * kCountersPerSlot];
+__device__ unsigned g_merge_counters[kCounterUsers * kCounterSlots * kCountersPerSlot];
 
 __device__ __forceinline__ float wave_max(float x) {
 #pragma unroll
@@ -1202,9 +1204,9 @@ int group_queries(int group) {
 
 }  // namespace
 
-// Counter slot of g_merge_counters for the current device and `stream`,
+// Counter slot of g_merge_counters for `user`, the current device and `stream`,
 // claimed on first use and kept; nullptr (decode: the two-launch path;
-// prefill: whole items) when n_bh counters exceed a slot or every slot is
+// prefill: whole items; attend_paged: counters in its workspace) when n_bh counters exceed a slot or every slot is
 // taken. The split-K decode and the split prefill units share a stream's
 // slot: kernels on one stream run one at a time, and each leaves its
 // counters at zero.
@@ -1215,7 +1217,7 @@ int group_queries(int group) {
 //    its capture id): graphs captured one after another on one stream (as
 //    torch.cuda.graph does) hold different slots and may replay concurrently.
 //    Replays of one graph share its slot and must not overlap each other.
-unsigned *merge_counters(hipStream_t stream, size_t n_bh) {
+unsigned *merge_counters(CounterUser user, hipStream_t stream, size_t n_bh) {
   if (n_bh > static_cast<size_t>(kCountersPerSlot)) return nullptr;
   if (stream == hipStreamPerThread || stream == hipStreamLegacy) return nullptr;
   int dev = 0;
@@ -1235,8 +1237,11 @@ unsigned *merge_counters(hipStream_t stream, size_t n_bh) {
   static std::mutex mu;
   static unsigned *base[kMaxDevices];
   static bool looked_up[kMaxDevices];
-  static Owner owner[kCounterSlots];
-  static int n_used = 0;
+  struct Slots {
+    Owner owner[kCounterSlots];
+    int n_used;
+  };
+  static Slots slots[kCounterUsers];
   std::lock_guard<std::mutex> lock(mu);
   if (!looked_up[dev]) {
     looked_up[dev] = true;
@@ -1245,12 +1250,16 @@ unsigned *merge_counters(hipStream_t stream, size_t n_bh) {
       base[dev] = static_cast<unsigned *>(p);
   }
   if (base[dev] == nullptr) return nullptr;
-  for (int i = 0; i < n_used; ++i)
-    if (owner[i].dev == dev && owner[i].stream == stream && owner[i].capture == capture)
-      return base[dev] + static_cast<size_t>(i) * kCountersPerSlot;
-  if (n_used == kCounterSlots) return nullptr;
-  owner[n_used] = {dev, stream, capture};
-  return base[dev] + static_cast<size_t>(n_used++) * kCountersPerSlot;
+  Slots &mine = slots[user];
+  unsigned *const first =
+      base[dev] + static_cast<size_t>(user) * kCounterSlots * kCountersPerSlot;
+  for (int i = 0; i < mine.n_used; ++i)
+    if (mine.owner[i].dev == dev && mine.owner[i].stream == stream &&
+        mine.owner[i].capture == capture)
+      return first + static_cast<size_t>(i) * kCountersPerSlot;
+  if (mine.n_used == kCounterSlots) return nullptr;
+  mine.owner[mine.n_used] = {dev, stream, capture};
+  return first + static_cast<size_t>(mine.n_used++) * kCountersPerSlot;
 }
 
 bool decode_needs_workspace(int batch, int heads, int kv_heads, int max_seq) {
@@ -1354,7 +1363,7 @@ int launch_valu_decode(const void *q, const void *k_cache, const void *v_cache,
   // chunks of up to 256 rows, where the per-chunk merge traffic and counter
   // contention dominate; 2 for longer chunks, where more blocks stream).
   // Else the split pass, then the merge pass.
-  unsigned *const counters = merge_counters(stream, bh);
+  unsigned *const counters = merge_counters(kAttentionCounters, stream, bh);
   if (counters != nullptr) {
     const int w = split_size <= 256 ? 4 : 2;
     const int n_groups = (n_splits + w - 1) / w;

@@ -1445,7 +1445,7 @@ int launch_attend_paged(AttendPagedParams p, bool bf16, int head_dim, float scal
                                          counter_bytes(static_cast<size_t>(n_blocks)));
   // Arrival counters: the stream's own, zero between calls, or, where it has no slot,
   // the workspace's, zeroed by a launch of their own.
-  p.counters = merge_counters(stream, static_cast<size_t>(n_blocks));
+  p.counters = merge_counters(kPagedCounters, stream, static_cast<size_t>(n_blocks));
   if (p.counters == nullptr) {
     p.counters = static_cast<unsigned *>(workspace);
     hipLaunchKernelGGL(zero_counters_kernel, dim3(static_cast<unsigned>((n_blocks + 255) / 256)),

@@ -1480,7 +1480,7 @@ void launch_one(const void *q, const void *k, const void *v, void *o, int bh,
   // one block per item.
   unsigned *counters = nullptr;
   if (planned && workspace != nullptr && workspace_bytes >= plan_workspace_bytes<D>(*e))
-    counters = merge_counters(stream, static_cast<size_t>(kRowWaves) * e->n_splits);
+    counters = merge_counters(kAttentionCounters, stream, static_cast<size_t>(kRowWaves) * e->n_splits);
   const auto *qp = static_cast<const _Float16 *>(q);
   const auto *kp = static_cast<const _Float16 *>(k);
   const auto *vp = static_cast<const _Float16 *>(v);

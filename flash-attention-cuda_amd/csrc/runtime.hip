@@ -14,6 +14,7 @@
 #include <mutex>
 
 #include "fa_internal.h"
+#include "flashattn_hip/paged.h"
 
 // Split-K partials of fa_decode_hd_noalloc: one copy of this array per
 // device, part of the library's code object, held until the process ends.

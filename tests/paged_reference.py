@@ -1,11 +1,21 @@
 """Plain 64-bit forms of rope, append_paged and attend_paged, on the CPU, with the
-error bounds their kernels have to meet."""
+error bounds their kernels have to meet, and the structures of their C entry points."""
 
-import math
+import ctypes
 
 import torch
 
-LOG2E = 1.0 / math.log(2.0)
+class Paged(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p)
+                 for n in ("k_pages", "v_pages", "page_table", "seq_lens", "cu_tokens")]
+                + [(n, ctypes.c_int)
+                   for n in ("dtype", "batch", "tokens", "kv_heads", "head_dim", "page_size",
+                             "num_pages", "max_pages")])
+
+
+class Rows(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64)]
 
 
 def half_step(dtype):

@@ -1,11 +1,15 @@
 """The paged cache: ``append_paged`` and ``attend_paged`` against plain forms in
 64 bits, at the sizes, lengths and contents where they can go wrong."""
 
+import ctypes
+import os
+
 import pytest
 import torch
 
 import flashattn_cuda
 import paged_reference as ref
+from paged_reference import Paged, Rows
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.float16, torch.bfloat16]
@@ -392,24 +396,62 @@ def test_a_captured_step_replays(dtype):
             assert torch.equal(a, b)
 
 
-def test_many_empty_sequences_and_more_streams_than_counters():
-    """Thousands of sequences without tokens around a few with them; the calls run
-    on fresh captures until the library has no arrival counters left for one, and
-    keep their results."""
+def test_many_empty_sequences():
+    """Thousands of sequences without tokens around a few with them."""
     sequences = [(0, 0)] * 3000 + [(2900, 3), (40, 1)] + [(0, 0)] * 2000 + [(700, 40)] + [(0, 0)] * 999
-    s = ref.batch(sequences, 1, 4, 64, 16, torch.float16, 21)
+    _check(ref.batch(sequences, 1, 4, 64, 16, torch.float16, 21))
+
+
+def test_a_stream_without_arrival_counters():
+    """hipStreamPerThread names another stream in every thread, so the library keeps no
+    counters for it and zeroes some in the workspace: same results, call after call."""
+    s = ref.batch([(3001, 40), (10, 1), (6100, 1)], 1, 4, 64, 16, torch.float16, 24)
     want = _attend(s, 0.125)
-    check, bound = ref.attend(s["q"], *(s[name] for name in CACHE), 0.125)
-    assert ((want.cpu().double() - check).abs() <= bound).all()
-    args = s["q"].cuda(), *(s[name].cuda() for name in CACHE), 0.125
+    t = {n: x.cuda() for n, x in s.items()}
+    lib = ctypes.CDLL(os.path.join(os.path.dirname(flashattn_cuda.__file__), "libflashattn_hip.so"))
+    lib.fa_attend_paged_workspace_bytes.restype = ctypes.c_size_t
+    tokens, heads, dim = t["q"].shape
+    cache = Paged(*(t[n].data_ptr() for n in CACHE), 0, len(t["seq_lens"]), tokens, 1, dim, 16,
+                  t["k_pages"].shape[0], t["page_table"].shape[1])
+    rows = Rows(t["q"].data_ptr(), t["q"].stride(0), t["q"].stride(1))
+    need = lib.fa_attend_paged_workspace_bytes(tokens, heads, 1, dim)
+    workspace = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+    out = [torch.empty_like(t["q"]) for _ in range(3)]
+    torch.cuda.synchronize()
+    for o in out:
+        assert lib.fa_attend_paged(ctypes.byref(cache), ctypes.byref(rows),
+                                   ctypes.c_void_p(o.data_ptr()), heads, ctypes.c_float(0.125),
+                                   ctypes.c_void_p(workspace.data_ptr()), ctypes.c_size_t(need),
+                                   ctypes.c_void_p(2)) == 0
+    torch.cuda.synchronize()  # every stream, the per-thread one included
+    assert all(torch.equal(o, want) for o in out)
+    # A workspace one byte short is refused.
+    assert lib.fa_attend_paged(ctypes.byref(cache), ctypes.byref(rows),
+                               ctypes.c_void_p(out[0].data_ptr()), heads, ctypes.c_float(0.125),
+                               ctypes.c_void_p(workspace.data_ptr()), ctypes.c_size_t(need - 1),
+                               None) == 2
+
+
+def test_more_captures_than_counter_slots():
+    """Every capture takes a slot of arrival counters until none is left; the graphs
+    captured after that zero counters in their workspace. All replay to the same bits."""
+    s = {n: t.cuda() for n, t in ref.batch([(2000, 40), (10, 1)], 1, 4, 64, 16, torch.float16,
+                                           26).items()}
+    want = _attend(s, 0.125)
+    graphs, outs = [], []
     for _ in range(70):
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
-            out = flashattn_cuda.attend_paged(*args)
-        graph.replay()
-        graph.replay()
+            outs.append(_attend(s, 0.125))
+        graphs.append(graph)
+    for _ in range(3):
+        for out in outs:
+            out.zero_()
+        for graph in graphs:
+            graph.replay()
         torch.cuda.synchronize()
-        assert torch.equal(out, want)
+        assert all(torch.equal(out, want) for out in outs)
+        assert torch.equal(_attend(s, 0.125), want)
 
 
 def test_two_streams_at_once():

@@ -4,26 +4,19 @@ is never followed."""
 
 import ctypes
 import os
+import re
+import subprocess
 
 import pytest
 
 import flashattn_cuda
+from paged_reference import Paged, Rows
 
 LIB = ctypes.CDLL(os.path.join(os.path.dirname(flashattn_cuda.__file__), "libflashattn_hip.so"))
 LIB.fa_last_error.restype = ctypes.c_char_p
 LIB.fa_attend_paged_workspace_bytes.restype = ctypes.c_size_t
 P, I, F, L = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_int64
 ADDRESS = 1 << 20
-
-
-class Paged(ctypes.Structure):
-    _fields_ = ([(n, P) for n in ("k_pages", "v_pages", "page_table", "seq_lens", "cu_tokens")]
-                + [(n, I) for n in ("dtype", "batch", "tokens", "kv_heads", "head_dim",
-                                    "page_size", "num_pages", "max_pages")])
-
-
-class Rows(ctypes.Structure):
-    _fields_ = [("data", P), ("token_stride", L), ("head_stride", L)]
 
 
 GOOD = dict(k_pages=ADDRESS, v_pages=ADDRESS, page_table=ADDRESS, seq_lens=ADDRESS,
@@ -34,6 +27,27 @@ ROW = dict(data=ADDRESS, token_stride=256, head_stride=64)
 LIB.fa_rope.argtypes = [P, P, P, P] + [I] * 5 + [L] * 4 + [I, I, F, I, P]
 LIB.fa_append_paged.argtypes = [P, P, P, P, P, I, P, I, I, F, P]
 LIB.fa_attend_paged.argtypes = [P, P, P, I, F, P, ctypes.c_size_t, P]
+
+
+HEADER = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include",
+                      "flashattn_hip", "paged.h")
+
+
+def test_header_declares_what_the_library_exports():
+    text = re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
+    names = sorted(set(re.findall(r"\b(fa_\w+)\s*\(", text)))
+    assert names == ["fa_append_paged", "fa_attend_paged", "fa_attend_paged_workspace_bytes",
+                     "fa_rope"]
+    assert all(hasattr(LIB, n) for n in names)
+
+
+def test_header_stands_alone_in_c_with_these_structures(tmp_path):
+    source = tmp_path / "sizes.c"
+    source.write_text(f'''#include "{HEADER}"
+_Static_assert(sizeof(fa_paged) == {ctypes.sizeof(Paged)}, "fa_paged");
+_Static_assert(sizeof(fa_rows) == {ctypes.sizeof(Rows)}, "fa_rows");
+''')
+    subprocess.run(["gcc", "-std=c11", "-Wall", "-Werror", "-fsyntax-only", str(source)], check=True)
 
 
 def _refused(rc, message):
