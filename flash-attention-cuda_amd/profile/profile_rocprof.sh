@@ -44,7 +44,8 @@ if [[ $# -gt 0 ]]; then
   WORKLOADS=("$@")
 else
   WORKLOADS=(copy_1g prefill_c3 prefill_c2_causal prefill_c2_full prefill_large decode_c4 decode_c5 decode_gqa_c5
-             prefill_c3_d128 decode_c5_d128)
+             prefill_c3_d128 decode_c5_d128 rope_batch append_chunks attend_batch attend_long
+             attend_prompt attend_chunks)
   BENCH=1
 fi
 mkdir -p "${OUT}"

@@ -54,6 +54,21 @@ WORKLOADS = {
                        2 * 14 * 128 * 2 * 73374 + 2 * 32 * 14 * 128 * 2 + 128),
     "decode_gqa_c5": ("config 5 batch with 2 K/V heads (group 7): grouped decode",
                       "decode_group_kernel", "byte", 2 * 2 * 64 * 2 * 73374 + 2 * 32 * 14 * 64 * 2 + 128),
+    "rope_batch": ("rotary positions of B=8 H=32 S=4096 D=128 bf16, token-major rows in",
+                   "rope_kernel", "byte", 2 * 8 * 32 * 4096 * 128 * 2),
+    "append_chunks": ("3 chunks of 2048 tokens into pages of 64, H=32 H_kv=8 D=128 bf16, q and k turned",
+                      "append_paged_kernel", "byte", 2 * 6144 * (32 + 2 * 8) * 128 * 2),
+    "attend_batch": ("config 5 lengths over pages of 16, one token each: H=14 H_kv=2 D=64",
+                     "attend_paged_kernel", "byte",
+                     2 * 2 * 64 * 2 * 73374 + 2 * 32 * 14 * 64 * 2),
+    "attend_long": ("8 sequences of 1023 to 8191 keys over pages of 64, one token each: H=32 H_kv=8 D=128 bf16",
+                    "attend_paged_kernel", "byte",
+                    2 * 8 * 128 * 2 * 36856 + 2 * 8 * 32 * 128 * 2),
+    "attend_prompt": ("prompt of 4096 tokens over pages of 16, H=14 D=64",
+                      "attend_paged_kernel", "flop", 4.0 * 14 * 64 * 4096 * 4097 / 2),
+    "attend_chunks": ("4 chunks of 2048 tokens behind 6144 over pages of 64, H=32 H_kv=8 D=128 bf16",
+                      "attend_paged_kernel", "flop",
+                      4.0 * 4 * 32 * 128 * (2048 * 6144 + 2048 * 2049 / 2)),
     "copy_1g": ("1 GiB device copy (byte-counter calibration)", "copyBuffer", "byte",
                 2.0 * (1 << 30)),
 }
@@ -128,6 +143,56 @@ def _decode(batch, heads, lmax, lens=None, kv_every=1, d=64):
     _run([lambda s=s: call(q, s[0], s[1], rl, d ** -0.5) for s in sets])
 
 
+def _rope(batch, heads, seq, d):
+    import torch
+
+    import flashattn_cuda as fa
+
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn((batch, seq, heads, d), generator=g).bfloat16().cuda().transpose(1, 2)
+    positions = torch.arange(seq, dtype=torch.int32, device="cuda")
+    inv_freq, _ = fa.rope_frequencies(d, device="cuda")
+    _run([lambda: fa.rope(x, positions, inv_freq)])
+
+
+def _paged(lens, new, heads, kv_heads, d, page, dtype, append=False):
+    """attend_paged (or append_paged) of `new` tokens for each of the lengths (None: config 5's)."""
+    import torch
+
+    import flashattn_cuda as fa
+
+    g = torch.Generator().manual_seed(0)
+    lens = _decode_inputs(32, 1, 4096, d=d)[3].tolist() if lens is None else lens
+    pages = [-(-n // page) for n in lens]
+    table = torch.zeros((len(lens), max(pages)), dtype=torch.int32)
+    order = torch.randperm(sum(pages), generator=g).to(torch.int32)
+    at = 0
+    for b, n in enumerate(pages):
+        table[b, :n] = order[at:at + n]
+        at += n
+    shape = (sum(pages), kv_heads, page, d)
+    tokens = new * len(lens)
+    qkv = torch.randn((tokens, heads + 2 * kv_heads, d), generator=g).to(dtype).cuda()
+    q, k, v = qkv.split([heads, kv_heads, kv_heads], dim=1)
+    index = (table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(),
+             (torch.arange(len(lens) + 1, dtype=torch.int32) * new).cuda())
+    caches = [torch.randn(shape, generator=g).to(dtype).cuda() for _ in range(2)]
+    n = _copies(2 * caches[0].numel() * 2)
+    sets = [caches] + [[c.clone() for c in caches] for _ in range(n - 1)]
+    if append:
+        inv_freq, _ = fa.rope_frequencies(d, device="cuda")
+        _run([lambda s=s: fa.append_paged(s[0], s[1], k, v, *index, q=q, inv_freq=inv_freq)
+              for s in sets])
+    else:
+        _run([lambda s=s: fa.attend_paged(q, s[0], s[1], *index, d ** -0.5) for s in sets])
+
+
+def _attend(lens, new, heads, kv_heads, d, page, bf16=False, append=False):
+    import torch
+
+    _paged(lens, new, heads, kv_heads, d, page, torch.bfloat16 if bf16 else torch.float16, append)
+
+
 def _copy():
     import torch
 
@@ -146,6 +211,13 @@ RUNNERS = {
     "decode_c5": lambda: _decode(32, 14, 4096),
     "decode_gqa_c5": lambda: _decode(32, 14, 4096, kv_every=7),
     "decode_c5_d128": lambda: _decode(32, 14, 4096, d=128),
+    "rope_batch": lambda: _rope(8, 32, 4096, 128),
+    "append_chunks": lambda: _attend([2048] * 3, 2048, 32, 8, 128, 64, bf16=True, append=True),
+    "attend_batch": lambda: _attend(None, 1, 14, 2, 64, 16),
+    "attend_long": lambda: _attend([1024 * i - 1 for i in range(1, 9)], 1, 32, 8, 128, 64,
+                                   bf16=True),
+    "attend_prompt": lambda: _attend([4096], 4096, 14, 14, 64, 16),
+    "attend_chunks": lambda: _attend([8192] * 4, 2048, 32, 8, 128, 64, bf16=True),
     "copy_1g": _copy,
 }
 

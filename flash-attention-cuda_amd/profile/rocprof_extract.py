@@ -44,14 +44,15 @@ HBM_PEAK_BYTES = 8.0e12           # MI355X HBM3E
 COPY_BYTES = float(1 << 30)       # the calibration copy reads and writes 1 GiB
 
 
+_TYPES = {"DF16_": "_Float16", "DF16b": "__bf16", "f": "float"}
 _LITERAL_TYPES = {"b": "bool", "i": "int", "j": "unsigned", "l": "long", "m": "unsigned long"}
 
 
 def _demangle_nested(name: str) -> str | None:
     """The name part of `_ZN <source-name>+ [I <literal args> E] E ...` or
     `_Z <source-name> [I ... E] ...`, with integer and bool literal template
-    arguments (`Lb1E` -> true, `Li8E` -> 8): enough for this library's
-    kernels, whose argument lists the report drops anyway. None when the
+    arguments (`Lb1E` -> true, `Li8E` -> 8) or element types: enough for this
+    library's kernels, whose argument lists the report drops anyway. None when the
     name has another form."""
     i = 2
     nested = name.startswith("_ZN")
@@ -76,7 +77,14 @@ def _demangle_nested(name: str) -> str | None:
     if i < len(name) and name[i] == "I":
         args = []
         i += 1
-        while i < len(name) and name[i] == "L":
+        while i < len(name) and name[i] != "E":
+            plain = next((t for t in _TYPES if name.startswith(t, i)), None)
+            if plain is not None:
+                args.append(_TYPES[plain])
+                i += len(plain)
+                continue
+            if name[i] != "L":
+                return None
             j = name.find("E", i)
             if j < 0 or name[i + 1] not in _LITERAL_TYPES:
                 return None
@@ -98,6 +106,10 @@ def demangle(name: str) -> str:
     small literal-template demangler above; other names are unchanged."""
     if not name.startswith("_Z"):
         return name
+    if "DF16" in name:  # older tools take bf16's DF16b apart wrongly
+        own = _demangle_nested(name)
+        if own:
+            return own
     tool = shutil.which("c++filt")
     if tool is not None:
         out = subprocess.run([tool, name], capture_output=True, text=True,
