@@ -1146,12 +1146,12 @@ __device__ __forceinline__ void narrow_item(ParamsRef p, const Item &it,
   block_barrier();  // the exchange may be overwritten
 }
 
-// Joins a narrow item's pieces, first to last, and writes its rows. Eight pieces' loads
-// are in flight at a time (16: 15.7 us for 15.1 where items have about 8; 4 alike).
-template <typename T, int D>
+// Joins a narrow item's pieces, first to last, and writes its rows. kDeep pieces' loads are
+// in flight at a time: 8, but 16 where there are more than 8 pieces (32 ragged sequences
+// of up to 9 pieces 14.3 -> 14.0 us, two of 8k keys 16.7 -> 16.3; 16 for all: 15.7 for 15.1).
+template <typename T, int D, int kDeep>
 __device__ __forceinline__ void join_narrow(ParamsRef p, const Item &it,
                                             const Pieces &pc) {
-  constexpr int kDeep = 8;
   typedef T t2 __attribute__((ext_vector_type(2)));
   const int n = it.n * p.group * (D / 2);
   const int thread = 64 * it.wave + fresh_lane();
@@ -1355,7 +1355,10 @@ __global__ __launch_bounds__(kThreads, Geo<D>::kBlocks) void attend_paged_kernel
         float *exchange = reinterpret_cast<float *>(ring_mem);
         if (it.n * p.group <= 16) narrow_item<T, D, 1>(anew(params), it, ring, exchange, ml_mem);
         else narrow_item<T, D, 2>(anew(params), it, ring, exchange, ml_mem);
-        if (!whole && counts_last()) join_narrow<T, D>(anew(params), it, pc);
+        if (!whole && counts_last()) {
+          if (pc.count <= 8) join_narrow<T, D, 8>(anew(params), it, pc);
+          else join_narrow<T, D, 16>(anew(params), it, pc);
+        }
       } else {
         Rows<T, D> r;
         wide_item<T, D>(anew(params), it, ring, votes, r);
