@@ -41,7 +41,7 @@
 //
 // Measured (us per call among others; B sequences, H / H_kv heads, D head_dim):
 //   B1 H12 D64, 512 keys, one token             7.2   chain of a block's loads (6 us of GPU)
-//   B32 H14/2 D64, 4096 keys ragged, one token 14.1   2.5 TB/s: share 2 us, ~4 rounds of
+//   B32 H14/2 D64, 4096 keys ragged, one token 13.9   2.7 TB/s: share 2 us, ~4 rounds of
 //                                                     loads, publish and join 2 us
 //   B8 H32/8 D128 bf16, 8191 ragged, one token 31.5   4.8 TB/s of K and V: HBM
 //   B1 H14 D64, prompt of 4096                 53.1   566 TFLOP/s; MFMA 32 %, VALU 50 % busy

@@ -3,6 +3,7 @@
 
 import ctypes
 import os
+import threading
 
 import pytest
 import torch
@@ -469,6 +470,45 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+def test_host_threads_at_once():
+    """Threads on streams of their own, attending and appending to caches of their own."""
+    batches = [ref.batch([(3001 + i, 1), (100, 40), (10, 1)], 2, 4, 64, 16, torch.float16, 30 + i)
+               for i in range(4)]
+    want = [_attend(s, 0.125) for s in batches]
+    on_gpu = [{n: x.cuda() for n, x in s.items()} for s in batches]
+    torch.cuda.synchronize()
+    got = [[] for _ in batches]
+
+    def work(i):
+        s = on_gpu[i]
+        cache = [s[n] for n in CACHE]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                got[i].append(flashattn_cuda.attend_paged(s["q"], *cache, 0.125))
+            flashattn_cuda.append_paged(*cache[:2], s["k"], s["v"], *cache[2:])
+            got[i].append(flashattn_cuda.attend_paged(s["q"], *cache, 0.125))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(batches))]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    for i, s in enumerate(on_gpu):
+        assert len(got[i]) == 11 and all(torch.equal(x, want[i]) for x in got[i][:10])
+        assert torch.equal(got[i][10], flashattn_cuda.attend_paged(
+            s["q"], *(s[n] for n in CACHE), 0.125))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_sequences_that_share_pages(dtype):
+    """A common prefix is stored once, and one page stands twice in a table."""
+    s = ref.batch([(160, 1), (160, 33), (500, 3)], 2, 6, 128, 32, dtype, 25)
+    s["page_table"][1, :5] = s["page_table"][0, :5]
+    s["page_table"][2, 3] = s["page_table"][2, 9]
+    _check(s, 0.09)
 
 
 def test_no_tokens():
