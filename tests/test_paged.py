@@ -403,6 +403,15 @@ def test_many_empty_sequences():
     _check(ref.batch(sequences, 1, 4, 64, 16, torch.float16, 21))
 
 
+@pytest.mark.parametrize("before,between,after", [(0, 62, 0), (1, 63, 5), (64, 64, 64),
+                                                  (3, 127, 1), (70, 200, 130)])
+def test_runs_of_empty_sequences(before, between, after):
+    """Slots without tokens, cached lengths kept, before, between and behind those in use."""
+    idle = [(33, 0)]
+    _check(ref.batch(idle * before + [(90, 1)] + idle * between + [(20, 40)] + idle * between
+                     + [(700, 3)] + idle * after, 2, 4, 64, 16, torch.float16, 27))
+
+
 def test_a_stream_without_arrival_counters():
     """hipStreamPerThread names another stream in every thread, so the library keeps no
     counters for it and zeroes some in the workspace: same results, call after call."""
