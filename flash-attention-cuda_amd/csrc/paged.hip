@@ -631,7 +631,7 @@ __device__ __forceinline__ void load_slab(const char *base, const unsigned (&off
         "global_load_lds_dwordx4 %0, %4 nt\n\t"
         "global_load_lds_dwordx4 %1, %4 offset:1024 nt\n\t"
         "global_load_lds_dwordx4 %2, %4 offset:2048 nt\n\t"
-        "global_load_lds_dwordx4 %3, %4 offset:3072 nt"
+        "global_load_lds_dwordx4 %3, %4 offset:3*1024 nt"
         ::"v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base), "s"(m0)
         : "memory", "m0");
   else
@@ -640,7 +640,7 @@ __device__ __forceinline__ void load_slab(const char *base, const unsigned (&off
         "global_load_lds_dwordx4 %0, %4\n\t"
         "global_load_lds_dwordx4 %1, %4 offset:1024\n\t"
         "global_load_lds_dwordx4 %2, %4 offset:2048\n\t"
-        "global_load_lds_dwordx4 %3, %4 offset:3072"
+        "global_load_lds_dwordx4 %3, %4 offset:3*1024"
         ::"v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base), "s"(m0)
         : "memory", "m0");
 }
