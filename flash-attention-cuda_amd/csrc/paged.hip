@@ -21,9 +21,9 @@
 //            from seq_lens and cu_tokens (1 us: kernel arguments, lengths, a
 //            sum over the lanes, 32-bit arithmetic).
 //   merge  = an item that a share's border cuts leaves one fp32 partial (O, m,
-//            l) per share in the workspace; the block that finishes last joins
-//            them in the order of the shares, so results do not depend on timing
-//            (a second launch for it took 2.6 to 18.7 us).
+//            l) per share in the workspace. They are joined along a fixed tree (wide: in
+//            pairs, narrow: 16 at a time) by whichever block is there last, so results
+//            do not depend on timing (a second launch for it took 2.6 to 18.7 us).
 //
 // Block: 256 threads, 4 waves.
 //   wide item: wave w owns query rows [32 w, +32); the waves share 64-key K and V
@@ -832,69 +832,51 @@ __device__ __forceinline__ void wide_item(ParamsRef p, const Item &it,
   if (fresh_lane() == 0) votes[wave] = lost;
   block_barrier();
   if (votes[0] | votes[1] | votes[2] | votes[3]) wide_pass<T, D, true>(p, it, ring, r);
-
-  if (!has_rows) return;
-  const int out_lane = fresh_lane(), out_row = 32 * wave + (out_lane & 31);
-  if (it.slot < 0) {
-    write_rows<T, D>(p, it, out_row, out_lane >> 5, r.o, r.l[0]);
-  } else {
-    float *part = partial_of(p, it.slot, D) + wave * (32 * D) + 2 * out_lane;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-      for (int a = 0; a < 8; ++a)
-        publish2(part + (8 * i + a) * 128, r.o[i][2 * a], r.o[i][2 * a + 1]);
-    if (out_lane < 32)
-      publish2(partial_of(p, it.slot, D) + kWideRows * D + 2 * out_row, r.m, r.l[0]);
-  }
 }
 
-// o a + x b, both products rounded: the same bits wherever x came from.
+// Stores a wave's rows of a wide item as a partial: its accumulators, then (m, l) pairs.
+template <typename T, int D>
+__device__ __forceinline__ void publish_wide(ParamsRef p, const Item &it, int slot,
+                                             const Rows<T, D> &r) {
+  const int lane = fresh_lane(), wave = it.wave;
+  if (32 * wave >= it.n * p.group) return;
+  float *part = partial_of(p, slot, D) + wave * (32 * D) + 2 * lane;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int a = 0; a < 8; ++a)
+      publish2(part + (8 * i + a) * 128, r.o[i][2 * a], r.o[i][2 * a + 1]);
+  if (lane < 32)
+    publish2(partial_of(p, slot, D) + kWideRows * D + 2 * (32 * wave + lane), r.m, r.l[0]);
+}
+
+// o a + x b, both products rounded: the same bits whichever of the two came from the
+// workspace.
 __device__ __forceinline__ float fold(float o, float a, float x, float b) {
 #pragma clang fp contract(off)
   return o * a + x * b;
 }
 
-// Joins a wide item's pieces, first to last, and writes its rows. Piece `own` is the
-// block's, still in its registers; the others come from the workspace, at ~5 thousand
-// cycles each (32 KiB at head_dim 64, past the L2).
+// Joins a partial to a wave's rows.
 template <typename T, int D>
-__device__ __forceinline__ void join_wide(ParamsRef p, const Item &it,
-                                          const Pieces &pc, int own, const Rows<T, D> &r) {
+__device__ __forceinline__ void merge_wide(ParamsRef p, const Item &it, int slot, Rows<T, D> &r) {
   const int lane = fresh_lane(), wave = it.wave;
-  const int row = 32 * wave + (lane & 31);
   if (32 * wave >= it.n * p.group) return;
-  float m = -INFINITY, l = 0.f;
-  floatx16 o[D / 32];
+  const float *part = partial_of(p, slot, D);
+  const floatx2 ml = fetch2(part + kWideRows * D + 2 * (32 * wave + (lane & 31)));
+  floatx2 x[D / 4];
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i)
+  for (int i = 0; i < D / 4; ++i) x[i] = fetch2(part + wave * (32 * D) + 128 * i + 2 * lane);
+  const float top = fmaxf(r.m, ml[0]);
+  const float a = r.m == -INFINITY ? 0.f : fast_exp2(r.m - top);
+  const float b = ml[0] == -INFINITY ? 0.f : fast_exp2(ml[0] - top);
+  r.m = top;
+  r.l[0] = fold(r.l[0], a, ml[1], b);
 #pragma unroll
-    for (int a = 0; a < 16; ++a) o[i][a] = 0.f;
-  for (int j = 0; j < pc.count; ++j) {
-    floatx2 ml = {r.m, r.l[0]};
-    floatx2 x[D / 4];
-    if (j == own) {
-#pragma unroll
-      for (int i = 0; i < D / 4; ++i)
-        x[i] = floatx2{r.o[i / 8][2 * (i % 8)], r.o[i / 8][2 * (i % 8) + 1]};
-    } else {
-      const float *part = partial_of(p, 2 * (pc.first + j - 1) + (j == 0 ? 1 : 0), D);
-      ml = fetch2(part + kWideRows * D + 2 * row);
-#pragma unroll
-      for (int i = 0; i < D / 4; ++i) x[i] = fetch2(part + wave * (32 * D) + 128 * i + 2 * lane);
-    }
-    const float top = fmaxf(m, ml[0]);
-    const float a = m == -INFINITY ? 0.f : fast_exp2(m - top);
-    const float b = ml[0] == -INFINITY ? 0.f : fast_exp2(ml[0] - top);
-    m = top;
-    l = fold(l, a, ml[1], b);
-#pragma unroll
-    for (int i = 0; i < D / 4; ++i) {
-      o[i / 8][2 * (i % 8)] = fold(o[i / 8][2 * (i % 8)], a, x[i][0], b);
-      o[i / 8][2 * (i % 8) + 1] = fold(o[i / 8][2 * (i % 8) + 1], a, x[i][1], b);
-    }
+  for (int i = 0; i < D / 4; ++i) {
+    r.o[i / 8][2 * (i % 8)] = fold(r.o[i / 8][2 * (i % 8)], a, x[i][0], b);
+    r.o[i / 8][2 * (i % 8) + 1] = fold(r.o[i / 8][2 * (i % 8) + 1], a, x[i][1], b);
   }
-  write_rows<T, D>(p, it, row, lane >> 5, o, l);
 }
 
 // Narrow items run on v_mfma_f32_16x16x32, with NQ groups of 16 query rows: with the
@@ -1350,39 +1332,78 @@ __global__ __launch_bounds__(kThreads, Geo<D>::kBlocks) void attend_paged_kernel
     if (whole || it.kt1 > it.kt0) {
       it.slot = whole ? -1 : 2 * w + (it.kt0 == 0 ? 1 : 0);
       Pieces pc;
-      // A partial is stored before it is counted; the block that counts last sets the
-      // counter back to zero for the next call, and joins the pieces.
-      auto counts_last = [&] {
+      auto find_pieces = [&] {
         const int x0 = from + kvh * weight_before(p, s, t, item, t.count) +
                        weight_before(p, s, t, item, tile);
         const int x1 = x0 + weight_before(p, s, t, item, tile + 1) - weight_before(p, s, t, item, tile);
-        pc = pieces_of(p, t, item, x0, x1, tiles, share);
+        pc = pieces_of(p, t, item, x0, x1, key_tiles(it.end), share);
+      };
+      // Counts the block at a border (what it stored before is visible first) and returns
+      // how many have been there; the `of`-th sets the counter back to zero for the next call.
+      auto count_at = [&](int border, int of) {
         wait_loads<0>();
         __syncthreads();
         if (wave == 0 && fresh_lane() == 0) {
-          unsigned *counter = p.counters + pc.first;
+          unsigned *counter = p.counters + border;
           arrived = 1 + static_cast<int>(__hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED,
                                                                 __HIP_MEMORY_SCOPE_AGENT));
-          if (arrived == pc.count)
+          if (arrived == of)
             __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
         __syncthreads();
-        return arrived == pc.count;
+        return arrived;
       };
       if (it.n * p.group <= kNarrowRows) {
         float *exchange = reinterpret_cast<float *>(ring_mem);
         if (it.n * p.group <= 16) narrow_item<T, D, 1>(anew(params), it, ring, exchange, ml_mem);
         else narrow_item<T, D, 2>(anew(params), it, ring, exchange, ml_mem);
-        if (!whole && counts_last()) {
+        if (it.slot >= 0) find_pieces();
+        if (it.slot >= 0 && count_at(pc.first, pc.count) == pc.count) {
           if (pc.count <= 8) join_narrow<T, D, 8>(anew(params), it, pc);
           else join_narrow<T, D, 16>(anew(params), it, pc);
         }
       } else {
         Rows<T, D> r;
         wide_item<T, D>(anew(params), it, ring, votes, r);
-        if (!whole && counts_last()) join_wide<T, D>(anew(params), it, pc, w - pc.first + 1, r);
+        // A cut item's pieces are joined in pairs, the pairs in pairs and so on, by the block
+        // of a pair that is there last: a fixed tree, so the order of arrival changes no
+        // bit. The other has left its rows in the slot of its first piece. Each pair counts
+        // at a border of its own, between its halves; a block that finds the other half
+        // there need not store its own. (All pieces by the last block, one by one, at ~2
+        // thousand cycles each: 16000 keys and 32 tokens of 14/2 heads 35.4 us for 26.7, 24
+        // sequences with 3 chunks 49.4 for 47.4, one token alike.)
+        bool holds = true;
+        if (it.slot >= 0) find_pieces();
+        else pc.count = 1;
+        for (int half = 1; half < pc.count; half *= 2) {
+          const int mine_from = (w - pc.first + 1) & -half, other = mine_from ^ half;
+          if (other >= pc.count) continue;
+          const int border = pc.first + max(mine_from, other) - 1;
+          auto slot_of = [&](int piece) { return 2 * (pc.first + piece - 1) + (piece == 0 ? 1 : 0); };
+          __syncthreads();  // `arrived` has been read
+          if (wave == 0 && fresh_lane() == 0) {
+            unsigned *counter = p.counters + border;
+            arrived = static_cast<int>(__hip_atomic_load(counter, __ATOMIC_RELAXED,
+                                                         __HIP_MEMORY_SCOPE_AGENT));
+            if (arrived != 0)
+              __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          }
+          __syncthreads();
+          if (arrived == 0) {
+            publish_wide<T, D>(anew(params), it, slot_of(mine_from), r);
+            if (count_at(border, 2) == 1) {
+              holds = false;
+              break;
+            }
+          }
+          merge_wide<T, D>(anew(params), it, slot_of(other), r);
+        }
+        if (holds && 32 * wave < it.n * p.group) {
+          const int lane = fresh_lane();
+          write_rows<T, D>(anew(params), it, 32 * wave + (lane & 31), lane >> 5, r.o, r.l[0]);
+        }
       }
-      if (!whole) __syncthreads();  // `arrived` may be written again
+      if (it.slot >= 0) __syncthreads();  // `arrived` may be written again
     }
     if (last) break;
     ++tile;
