@@ -83,6 +83,10 @@ constexpr int kMinShareKeys = 512;
 // such steps are never cut, since a cut costs about as much as two of them.
 constexpr int kWideStep = 2;
 constexpr int kWholeSteps = 4;
+// Narrow items of more pieces are joined in groups of 16 first (one sequence of 131072 keys of
+// 14/2 heads 42.2 -> 21.7 us, of 524288 82.4 -> 53.4; with 16 here two sequences of 17
+// pieces each 19.7 us for 16.3).
+constexpr int kFlatPieces = 48;
 
 // Blocks per CU and LDS for tiles per block, by head size. A head_dim 64 wave fits 168
 // VGPRs, so three blocks share a CU (two: prompt 57.3 us for 55.4, 20 sequences with 4
@@ -1187,6 +1191,78 @@ __device__ __forceinline__ void join_narrow(ParamsRef p, const Item &it,
   }
 }
 
+// Partials of a narrow item to join: partial j lies in slot `at` + j `step`, but the first in
+// `at0` and the last in `at1`. Piece i of an item (Pieces) is share first + i - 1's.
+struct NarrowJoin {
+  int count, at, step, at0, at1;
+};
+__device__ __forceinline__ int piece_slot(const Pieces &pc, int piece) {
+  return 2 * (pc.first + piece - 1) + (piece == 0 ? 1 : 0);
+}
+// Where the join of pieces [16 group, + 16) goes: to the second slot of a share that lies
+// within the item and so has no use for it, its first piece's, or its second one's where
+// that piece starts the item. A last group of one piece stays in that piece's slot.
+__device__ __forceinline__ int group_slot(const Pieces &pc, int group) {
+  return group == 0 ? 2 * pc.first + 1
+                    : 2 * (pc.first + 16 * group - 1) + (16 * group + 1 < pc.count ? 1 : 0);
+}
+
+// Joins them, in order, into slot `dest`, or into the output rows (dest < 0). A function of
+// its own beside join_narrow: one for both cost items of few pieces (32 ragged sequences
+// 15.0 us for 14.1).
+template <typename T, int D>
+__device__ __forceinline__ void join_many(ParamsRef p, const Item &it, const NarrowJoin &join,
+                                            int dest) {
+  constexpr int kDeep = 16;
+  int zero;  // per lane, so that the slots' addresses are not scalar: there are too many
+  asm volatile("v_mov_b32 %0, 0" : "=v"(zero));
+  typedef T t2 __attribute__((ext_vector_type(2)));
+  const int n = it.n * p.group * (D / 2), count = join.count;
+  const int thread = 64 * it.wave + fresh_lane();
+  for (int i = thread; i < n; i += kThreads) {
+    const int row = i / (D / 2), at = 2 * (i % (D / 2));
+    float m = -INFINITY, l = 0.f;
+    floatx2 o = {0.f, 0.f};
+    for (int j0 = 0; j0 < count; j0 += kDeep) {
+      floatx2 ml[kDeep], x[kDeep];
+#pragma unroll
+      for (int j = 0; j < kDeep; ++j) {
+        const int at_j = min(j0 + j, count - 1);
+        const int slot = at_j == 0 ? join.at0 : at_j == count - 1 ? join.at1
+                                                                  : join.at + at_j * join.step;
+        const float *part = partial_of(p, slot + zero, D);
+        ml[j] = fetch2(part + p.slot_rows * D + 2 * row);
+        x[j] = fetch2(part + row * D + at);
+      }
+      float top = m;
+#pragma unroll
+      for (int j = 0; j < kDeep; ++j) top = fmaxf(top, ml[j][0]);
+      const float base = top == -INFINITY ? 0.f : top;
+      const float old = fast_exp2(m - base);
+      m = top;
+      l *= old;
+      o *= old;
+#pragma unroll
+      for (int j = 0; j < kDeep; ++j) {
+        // A repeated last piece, or one whose keys the row does not see, counts for nothing.
+        const float a = j0 + j < count ? fast_exp2(ml[j][0] - base) : 0.f;
+        l += a == 0.f ? 0.f : a * ml[j][1];
+        o[0] += a == 0.f ? 0.f : a * x[j][0];
+        o[1] += a == 0.f ? 0.f : a * x[j][1];
+      }
+    }
+    if (dest >= 0) {
+      float *part = partial_of(p, dest, D);
+      publish2(part + row * D + at, o[0], o[1]);
+      if (at == 0) publish2(part + p.slot_rows * D + 2 * row, m, l);
+      continue;
+    }
+    const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
+    const t2 y = {static_cast<T>(o[0] * inv), static_cast<T>(o[1] * inv)};
+    *reinterpret_cast<t2 *>(out_row<T>(p, it.t0, it.kvh, row, D) + at) = y;
+  }
+}
+
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, Geo<D>::kBlocks) void attend_paged_kernel(const AttendPagedParams) {
   __shared__ __align__(1024) unsigned char ring_mem[Geo<D>::kRingBytes];
@@ -1358,9 +1434,38 @@ __global__ __launch_bounds__(kThreads, Geo<D>::kBlocks) void attend_paged_kernel
         if (it.n * p.group <= 16) narrow_item<T, D, 1>(anew(params), it, ring, exchange, ml_mem);
         else narrow_item<T, D, 2>(anew(params), it, ring, exchange, ml_mem);
         if (it.slot >= 0) find_pieces();
-        if (it.slot >= 0 && count_at(pc.first, pc.count) == pc.count) {
-          if (pc.count <= 8) join_narrow<T, D, 8>(anew(params), it, pc);
-          else join_narrow<T, D, 16>(anew(params), it, pc);
+        if (it.slot >= 0 && pc.count <= kFlatPieces) {
+          if (count_at(pc.first, pc.count) == pc.count) {
+            if (pc.count <= 8) join_narrow<T, D, 8>(anew(params), it, pc);
+            else join_narrow<T, D, 16>(anew(params), it, pc);
+          }
+        } else if (it.slot >= 0) {
+          // Groups of 16 pieces first, each counted at the border behind its first piece,
+          // then the groups.
+          const int group = (w - pc.first + 1) / 16;
+          NarrowJoin join;
+          join.count = min(pc.count - 16 * group, 16);
+          join.at0 = piece_slot(pc, 16 * group);
+          join.at = 2 * (pc.first + 16 * group - 1);
+          join.step = 2;
+          join.at1 = join.at + 2 * (join.count - 1);
+          int border = pc.first + 16 * group;
+          for (;;) {
+            const bool whole_item = join.step == 32;
+            if (join.count > 1) {
+              if (count_at(border, join.count) != join.count) break;
+              const int dest = whole_item ? -1 : group_slot(pc, group);
+              join_many<T, D>(anew(params), it, join, dest);
+              __syncthreads();  // `arrived` may be written again
+            }
+            if (whole_item) break;
+            join.count = (pc.count + 15) / 16;
+            join.at0 = group_slot(pc, 0);
+            join.at = 2 * (pc.first - 1) + 1;
+            join.step = 32;
+            join.at1 = group_slot(pc, join.count - 1);
+            border = pc.first + 15;
+          }
         }
       } else {
         Rows<T, D> r;

@@ -67,6 +67,28 @@ def test_attend_splits_long_contexts(dtype, dim):
     _check(ref.batch([(3001, 40), (10, 1), (4100, 1)], 1, 4, dim, 64, dtype, 4), dim ** -0.5)
 
 
+@pytest.mark.parametrize("dtype,dim", [(torch.float16, 64), (torch.bfloat16, 128)])
+@pytest.mark.parametrize("new", [1, 3, 40])
+@pytest.mark.parametrize("cached", [7900, 8300, 9000, 9600, 17000, 30000])
+def test_attend_joins_many_pieces(dtype, dim, new, cached):
+    """One long sequence: about 15 to 60 pieces of an item, 17 and 33 among them."""
+    _check(ref.batch([(cached, new)], 1, 5, dim, 64, dtype, cached % 89))
+
+
+def test_items_cut_anywhere_join_alike():
+    """Lengths that move every border, beside a neighbour in the same shares."""
+    for cached in range(9000, 12000, 131):
+        _check(ref.batch([(200, 2), (cached, 1), (150, 1), (cached - 2000, 33)], 1, 4, 64, 32,
+                         torch.float16, cached % 97))
+
+
+def test_joins_of_groups_of_pieces():
+    """Counts of pieces from under 48 to over 65: joined at once, or by 16 with a last group
+    of any size, one piece among them."""
+    for cached in range(24000, 35000, 509):
+        _check(ref.batch([(cached, 1 + cached % 2)], 1, 3, 64, 128, torch.float16, cached % 83))
+
+
 def test_attend_many_sequences():
     """More sequences than threads of a block."""
     gen = torch.Generator().manual_seed(5)
