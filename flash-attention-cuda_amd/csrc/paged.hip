@@ -40,13 +40,13 @@
 // 2.0e-4 (the output's own rounding); bf16 2.3e-3 and 1.7e-3.
 //
 // Measured (us per call among others; B sequences, H / H_kv heads, D head_dim):
-//   B1 H12 D64, 512 keys, one token             7.2   chain of a block's loads (6 us of GPU)
-//   B32 H14/2 D64, 4096 keys ragged, one token 13.9   2.7 TB/s: share 2 us, ~4 rounds of
+//   B1 H12 D64, 512 keys, one token             7.3   chain of a block's loads (6 us of GPU)
+//   B32 H14/2 D64, 4096 keys ragged, one token 14.0   2.7 TB/s: share 2 us, ~4 rounds of
 //                                                     loads, publish and join 2 us
-//   B8 H32/8 D128 bf16, 8191 ragged, one token 31.5   4.8 TB/s of K and V: HBM
-//   B1 H14 D64, prompt of 4096                 53.1   566 TFLOP/s; MFMA 32 %, VALU 50 % busy
-//   B24 H28/4 D128, 3 chunks to 777 + tokens   48.8   2.6 TB/s and 330 TFLOP/s
-//   B4 H32/8 D128 bf16, chunks to 2048 on 6144  482   936 TFLOP/s; MFMA 48 %, VALU 35 % busy:
+//   B8 H32/8 D128 bf16, 8191 ragged, one token 31.1   4.9 TB/s of K and V: HBM
+//   B1 H14 D64, prompt of 4096                 52.8   570 TFLOP/s; MFMA 32 %, VALU 50 % busy
+//   B24 H28/4 D128, 3 chunks to 777 + tokens   47.5   2.7 TB/s and 340 TFLOP/s
+//   B4 H32/8 D128 bf16, chunks to 2048 on 6144  484   932 TFLOP/s; MFMA 48 %, VALU 35 % busy:
 //                                                     the two hardly run at once
 //
 // Memory safety. Lengths, bounds and page ids are device data, which the host
