@@ -263,6 +263,10 @@ __device__ __forceinline__ void place_border(ParamsRef p, const Tiles &t, int it
 struct Pieces {
   int first, count;
 };
+// The workspace slot of a piece: a share may end one item and begin the next.
+__device__ __forceinline__ int piece_slot(const Pieces &pc, int piece) {
+  return 2 * (pc.first + piece - 1) + (piece == 0 ? 1 : 0);
+}
 __device__ __forceinline__ int ceil_units(ParamsRef p, int64_t keys) {
   return static_cast<int>((keys + (int64_t{1} << p.unit) - 1) >> p.unit);
 }
@@ -1163,8 +1167,7 @@ __device__ __forceinline__ void join_narrow(ParamsRef p, const Item &it,
 #pragma unroll
       for (int j = 0; j < kDeep; ++j) {
         const int piece = min(j0 + j, pc.count - 1);
-        const int share = pc.first + piece - 1;
-        const float *part = partial_of(p, 2 * share + (piece == 0 ? 1 : 0), D);
+        const float *part = partial_of(p, piece_slot(pc, piece), D);
         ml[j] = fetch2(part + p.slot_rows * D + 2 * row);
         x[j] = fetch2(part + row * D + at);
       }
@@ -1192,13 +1195,10 @@ __device__ __forceinline__ void join_narrow(ParamsRef p, const Item &it,
 }
 
 // Partials of a narrow item to join: partial j lies in slot `at` + j `step`, but the first in
-// `at0` and the last in `at1`. Piece i of an item (Pieces) is share first + i - 1's.
+// `at0` and the last in `at1`.
 struct NarrowJoin {
   int count, at, step, at0, at1;
 };
-__device__ __forceinline__ int piece_slot(const Pieces &pc, int piece) {
-  return 2 * (pc.first + piece - 1) + (piece == 0 ? 1 : 0);
-}
 // Where the join of pieces [16 group, + 16) goes: to the second slot of a share that lies
 // within the item and so has no use for it, its first piece's, or its second one's where
 // that piece starts the item. A last group of one piece stays in that piece's slot.
@@ -1484,7 +1484,6 @@ __global__ __launch_bounds__(kThreads, Geo<D>::kBlocks) void attend_paged_kernel
           const int mine_from = (w - pc.first + 1) & -half, other = mine_from ^ half;
           if (other >= pc.count) continue;
           const int border = pc.first + max(mine_from, other) - 1;
-          auto slot_of = [&](int piece) { return 2 * (pc.first + piece - 1) + (piece == 0 ? 1 : 0); };
           __syncthreads();  // `arrived` has been read
           if (wave == 0 && fresh_lane() == 0) {
             unsigned *counter = p.counters + border;
@@ -1495,13 +1494,13 @@ __global__ __launch_bounds__(kThreads, Geo<D>::kBlocks) void attend_paged_kernel
           }
           __syncthreads();
           if (arrived == 0) {
-            publish_wide<T, D>(anew(params), it, slot_of(mine_from), r);
+            publish_wide<T, D>(anew(params), it, piece_slot(pc, mine_from), r);
             if (count_at(border, 2) == 1) {
               holds = false;
               break;
             }
           }
-          merge_wide<T, D>(anew(params), it, slot_of(other), r);
+          merge_wide<T, D>(anew(params), it, piece_slot(pc, other), r);
         }
         if (holds && 32 * wave < it.n * p.group) {
           const int lane = fresh_lane();
