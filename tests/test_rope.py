@@ -68,6 +68,20 @@ def test_rope_takes_views_and_shared_positions(dtype):
 
 
 @gpu
+def test_rope_past_2_to_the_31_elements():
+    """The last heads of a tensor of 2^31 and more elements, and of a token-major view of it."""
+    inv_freq, _ = flashattn_cuda.rope_frequencies(128, device="cuda")
+    positions = torch.arange(1 << 19, dtype=torch.int32, device="cuda")
+    x = torch.empty((1, 33, 1 << 19, 128), dtype=torch.float16, device="cuda")
+    x[:, :31] = 0
+    x[:, 31:] = torch.randn((1, 2, 1 << 19, 128), device="cuda", dtype=torch.float16)
+    want = flashattn_cuda.rope(x[:, 31:].contiguous(), positions, inv_freq)
+    assert torch.equal(flashattn_cuda.rope(x, positions, inv_freq)[:, 31:], want)
+    tokens = x.transpose(1, 2).contiguous().transpose(1, 2)
+    assert torch.equal(flashattn_cuda.rope(tokens, positions, inv_freq)[:, 31:], want)
+
+
+@gpu
 def test_rope_of_no_rows_is_empty():
     inv_freq = flashattn_cuda.rope_frequencies(64)[0].cuda()
     for shape in [(0, 2, 5, 64), (2, 0, 5, 64), (2, 2, 0, 64)]:
