@@ -34,22 +34,14 @@ HEADS = [(12, 12), (14, 14), (8, 8), (14, 2), (32, 8), (28, 4)]
 DTYPES = {"fp16": torch.float16, "bf16": torch.bfloat16}
 
 
-_imported = None
-
-
 def _package():
-    """The package, imported at the first call (a program imports it once)."""
-    global _imported
-    if _imported is not None:
-        return _imported
     path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
                         "flash-attention-cuda_amd")
     if path not in sys.path:
         sys.path.insert(0, path)
     import flashattn_cuda
 
-    _imported = flashattn_cuda
-    return _imported
+    return flashattn_cuda
 
 
 # ---- cases --------------------------------------------------------------------
