@@ -192,8 +192,9 @@ __global__ __launch_bounds__(kRopeThreads) void append_paged_kernel(const Append
   const int h0 = static_cast<int>(blockIdx.y) * p.heads_per_thread;
   const int h1 = min(h0 + p.heads_per_thread, p.q_heads + 2 * p.kv_heads);
 
+  // Tokens in front of the first sequence's count as its own there.
   const int b = sequence_of(p.cu_tokens, p.batch, t);
-  const bool live = b < p.batch;
+  const bool live = b < p.batch && t >= p.cu_tokens[b];
   int64_t pos = 0;
   int64_t row = -1;  // row of the token in the page pool, counted over (page, row) pairs
   if (live) {
@@ -228,7 +229,7 @@ __global__ __launch_bounds__(kRopeThreads) void append_paged_kernel(const Append
     V a = *reinterpret_cast<const V *>(src + at.first);
     V c = *reinterpret_cast<const V *>(src + at.second);
     if (vh < 0 && at.turned) turn<T>(a, c, turns, p.interleaved);
-    if (!live) a = c = V{};  // a query row behind the last sequence
+    if (!live) a = c = V{};  // a query row outside every sequence
     store_piece<true>(reinterpret_cast<V *>(dst + at.first), a);
     store_piece<true>(reinterpret_cast<V *>(dst + at.second), c);
   }

@@ -71,7 +71,8 @@ typedef struct fa_rows {
  * [tokens, H, head_dim] (rows that belong to no sequence become zero); with
  * rotary_dim 0, q, q_out and inv_freq are not used. Lengths are not changed: the
  * call can be repeated. No two tokens may have the same place, and q_out overlaps
- * no input. */
+ * no input. Where cu_tokens falls, a token still goes to one sequence at most, whose
+ * bounds hold it, and to its place among that one's new tokens. */
 int fa_append_paged(const fa_paged *cache, const fa_rows *k, const fa_rows *v, const fa_rows *q,
                     void *q_out, int heads, const double *inv_freq, int rotary_dim,
                     int interleaved, float factor, void *stream);
