@@ -1149,19 +1149,52 @@ __device__ __forceinline__ void narrow_item(ParamsRef p, const Item &it,
   block_barrier();  // the exchange may be overwritten
 }
 
+// Two dims of a narrow item's row, joined from its partials.
+struct JoinedRow {
+  float m = -INFINITY, l = 0.f;
+  floatx2 o = {0.f, 0.f};
+
+  // Joins the first `fresh` of kDeep partials (the others repeat the last one). One without a
+  // key that the row sees has l = 0 and o = 0. None is left out for a weight of zero: a NaN or
+  // an infinity that the row does see stays in it (0 * inf), as in an item that is not cut.
+  template <int kDeep>
+  __device__ __forceinline__ void fold(const floatx2 (&ml)[kDeep], const floatx2 (&x)[kDeep],
+                                       int fresh) {
+    float top = m;
+#pragma unroll
+    for (int j = 0; j < kDeep; ++j) top = fmaxf(top, ml[j][0]);
+    const float base = top == -INFINITY ? 0.f : top;
+    const float old = fast_exp2(m - base);
+    m = top;
+    l *= old;
+    o *= old;
+#pragma unroll
+    for (int j = 0; j < kDeep; ++j) {
+      const float a = fast_exp2(ml[j][0] - base);
+      l += j < fresh ? a * ml[j][1] : 0.f;
+      o[0] += j < fresh ? a * x[j][0] : 0.f;
+      o[1] += j < fresh ? a * x[j][1] : 0.f;
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ void write(T *out) const {
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;  // NaN stays NaN
+    *reinterpret_cast<t2 *>(out) = t2{static_cast<T>(o[0] * inv), static_cast<T>(o[1] * inv)};
+  }
+};
+
 // Joins a narrow item's pieces, first to last, and writes its rows. kDeep pieces' loads are
 // in flight at a time: 8, but 16 where there are more than 8 pieces (32 ragged sequences
 // of up to 9 pieces 14.3 -> 14.0 us, two of 8k keys 16.7 -> 16.3; 16 for all: 15.7 for 15.1).
 template <typename T, int D, int kDeep>
 __device__ __forceinline__ void join_narrow(ParamsRef p, const Item &it,
                                             const Pieces &pc) {
-  typedef T t2 __attribute__((ext_vector_type(2)));
   const int n = it.n * p.group * (D / 2);
   const int thread = 64 * it.wave + fresh_lane();
   for (int i = thread; i < n; i += kThreads) {
     const int row = i / (D / 2), at = 2 * (i % (D / 2));
-    float m = -INFINITY, l = 0.f;
-    floatx2 o = {0.f, 0.f};
+    JoinedRow r;
     for (int j0 = 0; j0 < pc.count; j0 += kDeep) {
       floatx2 ml[kDeep], x[kDeep];
 #pragma unroll
@@ -1171,26 +1204,9 @@ __device__ __forceinline__ void join_narrow(ParamsRef p, const Item &it,
         ml[j] = fetch2(part + p.slot_rows * D + 2 * row);
         x[j] = fetch2(part + row * D + at);
       }
-      float top = m;
-#pragma unroll
-      for (int j = 0; j < kDeep; ++j) top = fmaxf(top, ml[j][0]);
-      const float base = top == -INFINITY ? 0.f : top;
-      const float old = fast_exp2(m - base);
-      m = top;
-      l *= old;
-      o *= old;
-#pragma unroll
-      for (int j = 0; j < kDeep; ++j) {
-        // A repeated last piece, or one whose keys the row does not see, counts for nothing.
-        const float a = j0 + j < pc.count ? fast_exp2(ml[j][0] - base) : 0.f;
-        l += a == 0.f ? 0.f : a * ml[j][1];
-        o[0] += a == 0.f ? 0.f : a * x[j][0];
-        o[1] += a == 0.f ? 0.f : a * x[j][1];
-      }
+      r.fold(ml, x, pc.count - j0);
     }
-    const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
-    const t2 y = {static_cast<T>(o[0] * inv), static_cast<T>(o[1] * inv)};
-    *reinterpret_cast<t2 *>(out_row<T>(p, it.t0, it.kvh, row, D) + at) = y;
+    r.write<T>(out_row<T>(p, it.t0, it.kvh, row, D) + at);
   }
 }
 
@@ -1216,13 +1232,11 @@ __device__ __forceinline__ void join_many(ParamsRef p, const Item &it, const Nar
   constexpr int kDeep = 16;
   int zero;  // per lane, so that the slots' addresses are not scalar: there are too many
   asm volatile("v_mov_b32 %0, 0" : "=v"(zero));
-  typedef T t2 __attribute__((ext_vector_type(2)));
   const int n = it.n * p.group * (D / 2), count = join.count;
   const int thread = 64 * it.wave + fresh_lane();
   for (int i = thread; i < n; i += kThreads) {
     const int row = i / (D / 2), at = 2 * (i % (D / 2));
-    float m = -INFINITY, l = 0.f;
-    floatx2 o = {0.f, 0.f};
+    JoinedRow r;
     for (int j0 = 0; j0 < count; j0 += kDeep) {
       floatx2 ml[kDeep], x[kDeep];
 #pragma unroll
@@ -1234,32 +1248,15 @@ __device__ __forceinline__ void join_many(ParamsRef p, const Item &it, const Nar
         ml[j] = fetch2(part + p.slot_rows * D + 2 * row);
         x[j] = fetch2(part + row * D + at);
       }
-      float top = m;
-#pragma unroll
-      for (int j = 0; j < kDeep; ++j) top = fmaxf(top, ml[j][0]);
-      const float base = top == -INFINITY ? 0.f : top;
-      const float old = fast_exp2(m - base);
-      m = top;
-      l *= old;
-      o *= old;
-#pragma unroll
-      for (int j = 0; j < kDeep; ++j) {
-        // A repeated last piece, or one whose keys the row does not see, counts for nothing.
-        const float a = j0 + j < count ? fast_exp2(ml[j][0] - base) : 0.f;
-        l += a == 0.f ? 0.f : a * ml[j][1];
-        o[0] += a == 0.f ? 0.f : a * x[j][0];
-        o[1] += a == 0.f ? 0.f : a * x[j][1];
-      }
+      r.fold(ml, x, count - j0);
     }
     if (dest >= 0) {
       float *part = partial_of(p, dest, D);
-      publish2(part + row * D + at, o[0], o[1]);
-      if (at == 0) publish2(part + p.slot_rows * D + 2 * row, m, l);
+      publish2(part + row * D + at, r.o[0], r.o[1]);
+      if (at == 0) publish2(part + p.slot_rows * D + 2 * row, r.m, r.l);
       continue;
     }
-    const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
-    const t2 y = {static_cast<T>(o[0] * inv), static_cast<T>(o[1] * inv)};
-    *reinterpret_cast<t2 *>(out_row<T>(p, it.t0, it.kvh, row, D) + at) = y;
+    r.write<T>(out_row<T>(p, it.t0, it.kvh, row, D) + at);
   }
 }
 
