@@ -104,11 +104,16 @@ struct Geo<128> {
   static constexpr int kBlocks = 2, kRingBytes = 64 * 1024;
 };
 
+// kLift: a row's bound is put this many powers of two under the largest score that set it, so
+// its largest weight is 2^kLift or more there (and 2^(kLift + 8) at most, see weigh). fp16 has
+// places of 2^-24 and none below: at 0 the weights of a context's many small keys beside a
+// few large ones came out as 0 or 41 % over (16384 keys at 2^-24.5 of the largest).
 template <typename T>
 struct Frag;
 template <>
 struct Frag<_Float16> {
   typedef half8 type;
+  static constexpr float kLift = 7.0f;
   static __device__ __forceinline__ floatx16 mm(type a, type b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
@@ -119,6 +124,7 @@ struct Frag<_Float16> {
 template <>
 struct Frag<__bf16> {
   typedef __bf16 type __attribute__((ext_vector_type(8)));
+  static constexpr float kLift = 0.0f;
   static __device__ __forceinline__ floatx16 mm(type a, type b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -436,9 +442,9 @@ __device__ __forceinline__ void hide(floatx16 (&s)[KB], int lim, unsigned absent
     }
 }
 
-// Weights of the tile as P^T fragments. The bound m moves only when a row's scores pass it by
-// more than 2^8 (weights up to 2^8 are harmless in either type): O is rescaled a few times
-// per item instead of per tile.
+// Weights of the tile as P^T fragments. The bound m moves only when a row's scores pass the one
+// that set it by more than 2^8 (weights up to 2^(kLift + 8) fit either type): O is rescaled a
+// few times per item instead of per tile.
 template <typename T, int D, int KB>
 __device__ __forceinline__ void weigh(floatx16 (&s)[KB], float c, Rows<T, D> &r,
                                       frag_t<T> (&w)[2 * KB]) {
@@ -447,7 +453,7 @@ __device__ __forceinline__ void weigh(floatx16 (&s)[KB], float c, Rows<T, D> &r,
   for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
     for (int a = 0; a < 16; ++a) mx = fmaxf(mx, s[kb][a]);
-  mx = max_lane_pair(mx) * c;
+  mx = max_lane_pair(mx) * c - Frag<T>::kLift;
   if (__builtin_amdgcn_ballot_w64(mx > r.m + 8.0f) != 0) {
     const float m = fmaxf(r.m, mx);
     const float alpha = m == -INFINITY ? 1.0f : fast_exp2(r.m - m);
@@ -1005,7 +1011,7 @@ __device__ __forceinline__ void narrow_pass(ParamsRef p, const Item &it,
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int j = 0; j < 4; ++j) mx = fmaxf(mx, s[i][kb][j]);
-      mx = max_lane_groups(mx) * p.c;
+      mx = max_lane_groups(mx) * p.c - Frag<T>::kLift;
       if (__builtin_amdgcn_ballot_w64(mx > m[i] + 8.0f) != 0) {
         const float top = fmaxf(m[i], mx);
         const float alpha = top == -INFINITY ? 1.0f : fast_exp2(m[i] - top);

@@ -87,7 +87,8 @@ size_t fa_attend_paged_workspace_bytes(int tokens, int heads, int kv_heads, int 
  * [tokens, H, head_dim] and overlaps no input; a row without a key, and one that
  * belongs to no sequence, is zero; so is every row if cu_tokens rises and falls so
  * that the sequences claim more rows than there are. What a query does not see does not
- * reach it, infinities and NaN included. At most 128 query heads per K/V head.
+ * reach it, infinities and NaN included; what it sees does. Scores scale q . k are held in
+ * 32 bits: up to 10^7 either way. At most 128 query heads per K/V head.
  * Workspace and streams follow the rules of the split-K decode: the workspace stays
  * untouched until the launch completes, calls on one stream are ordered, replays of
  * one graph must not overlap. */
