@@ -162,7 +162,8 @@ __device__ __forceinline__ uniform_ints uniform_at(const int32_t *p) {
   return (uniform_ints)(reinterpret_cast<uintptr_t>(p));
 }
 
-// A sequence's new tokens: packed rows [t0, t0 + n), the first at position p0.
+// A sequence's new tokens: packed rows [t0, t0 + n), the first at position p0. n is below 0
+// where its bounds fall within the packed rows.
 struct Seq {
   int t0, n, p0;
 };
@@ -171,7 +172,7 @@ __device__ __forceinline__ Seq load_seq(ParamsRef p, Ints bounds, Ints lens, int
   const int lo = bounds[b], hi = bounds[b + 1];
   Seq s;
   s.t0 = min(max(lo, 0), p.tokens);
-  s.n = min(max(hi, s.t0), p.tokens) - s.t0;
+  s.n = min(max(hi, 0), p.tokens) - s.t0;
   // lens[b] - hi + t0, kept far from overflow whatever the buffers hold.
   const int64_t p0 = static_cast<int64_t>(lens[b]) - hi + s.t0;
   s.p0 = static_cast<int>(min(max(p0, static_cast<int64_t>(-(1 << 30))),
@@ -1294,7 +1295,7 @@ __global__ __launch_bounds__(kThreads, Geo<D>::kBlocks) void attend_paged_kernel
   // Every wave sums the sequences' weights (lane l takes `per` of them) and finds its
   // block's two borders: no exchange between waves, and scalar code from there on.
   const int per = (p.batch + kWave - 1) / kWave;
-  int mine = 0, my_items = 0, my_tokens = 0;
+  int mine = 0, my_items = 0, signs = 0;
   Seq s = {0, 0, 0};
   for (int i = 0; i < per; ++i) {
     const int b = lane * per + i;
@@ -1303,12 +1304,12 @@ __global__ __launch_bounds__(kThreads, Geo<D>::kBlocks) void attend_paged_kernel
     const Tiles t = tiles_of<false>(p, s.n);
     mine += keys_before(p, s, t, t.count) * p.kv_heads;
     my_items += t.count * p.kv_heads;
-    my_tokens = min(my_tokens + s.n, p.tokens + 1);
+    signs |= s.n;
   }
   const int keys_upto = wave_prefix(mine), items_upto = wave_prefix(my_items);
-  // Bounds that go up and down can claim more rows than there are, beyond what the weights'
-  // 30 bits were chosen for: such a batch has no sequences, and its outputs are zero.
-  const bool sound = __builtin_amdgcn_readlane(wave_prefix(my_tokens), kWave - 1) <= p.tokens;
+  // Bounds that go up and down can claim a row twice, or more rows than there are, beyond what
+  // the weights' 30 bits were chosen for: such a batch has no sequences, and its outputs are zero.
+  const bool sound = __builtin_amdgcn_ballot_w64(signs < 0) == 0;
   const int tail = sound ? last_bound : 0;
   const int all_keys = __builtin_amdgcn_readlane(keys_upto, kWave - 1);
   const int all_items = __builtin_amdgcn_readlane(items_upto, kWave - 1);

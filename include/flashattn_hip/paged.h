@@ -85,8 +85,8 @@ size_t fa_attend_paged_workspace_bytes(int tokens, int heads, int kv_heads, int 
  * (written before) among it: o[t, h] = softmax over keys 0..position(t) of
  * scale * q[t, h] . k, times v, with K/V head h / (H / H_kv). out is contiguous
  * [tokens, H, head_dim] and overlaps no input; a row without a key, and one that
- * belongs to no sequence, is zero; so is every row if cu_tokens rises and falls so
- * that the sequences claim more rows than there are. What a query does not see does not
+ * belongs to no sequence, is zero; so is every row if cu_tokens falls anywhere
+ * within the packed rows. What a query does not see does not
  * reach it, infinities and NaN included; what it sees does. Scores scale q . k are held in
  * 32 bits: up to 10^7 either way. At most 128 query heads per K/V head.
  * Workspace and streams follow the rules of the split-K decode: the workspace stays

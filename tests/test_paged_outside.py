@@ -108,3 +108,55 @@ def test_both_calls_agree_on_what_is_outside(front):
         assert torch.equal(outs[1][i][front:], outs[0][i])
     for i in (1, 2):
         assert torch.equal(outs[1][i], outs[0][i])
+
+
+def _attend(s):
+    return flashattn_cuda.attend_paged(s["q"].cuda(), *(s[n].cuda() for n in CACHE), 0.125).cpu()
+
+
+@pytest.mark.parametrize("dtype,kv_heads,heads", [(torch.float16, 2, 4), (torch.bfloat16, 1, 40)])
+def test_bounds_that_fall_give_no_row_to_two_sequences(dtype, kv_heads, heads):
+    """A fall by one row or more, first, last or among many, also where the sequences claim no
+    more rows than there are: zeros, and the next call is as if nothing had been."""
+    for bounds, tokens in (([0, 5, 3, 4], 8), ([0, 5, 4, 4], 9), ([3, 2, 8, 8], 8),
+                           ([0, 2, 4, 6, 8, 7], 8), ([0, 70, 60, 65], 200),
+                           (list(range(150)) + [140] + [141] * 49, 150)):
+        s = ref.batch([(40, 1)] * (len(bounds) - 1), kv_heads, heads, 64, 16, dtype, 63)
+        s["q"] = torch.randn(tokens, heads, 64, generator=torch.Generator().manual_seed(1)).to(dtype)
+        s["cu_tokens"] = torch.tensor(bounds, dtype=torch.int32)
+        assert (_attend(s) == 0).all(), bounds
+        s["cu_tokens"] = torch.tensor(bounds, dtype=torch.int32).cummax(0)[0].to(torch.int32)
+        want, bound = ref.attend(s["q"], *(s[n] for n in CACHE), 0.125)
+        assert ((_attend(s).double() - want).abs() <= bound).all(), bounds
+
+
+def test_bounds_that_fall_outside_the_rows_are_those_of_its_ends():
+    """Bounds past the packed rows, or below them, end there; falls among them claim nothing."""
+    s = ref.batch([(40, 5), (20, 3), (30, 0), (9, 0)], 2, 4, 64, 16, torch.float16, 64)
+    want = _attend(s)
+    s["cu_tokens"] = torch.tensor([0, 5, 8, 30, 12], dtype=torch.int32)
+    assert torch.equal(_attend(s), want)
+    # The first two sequences have no rows; the third's bounds are [-1, 5).
+    s["cu_tokens"] = torch.tensor([-1, -9, -1, 5, 8], dtype=torch.int32)
+    want, bound = ref.attend(s["q"], s["k_pages"], s["v_pages"], s["page_table"],
+                             s["seq_lens"], s["cu_tokens"].clamp(min=0), 0.125)
+    assert ((_attend(s).double() - want).abs() <= bound).all()
+
+
+def test_append_with_bounds_that_fall():
+    """A token goes to its place in a sequence whose bounds hold it, or nowhere; nothing but
+    the last seq_len - n.. rows of the sequences changes."""
+    s = ref.batch([(40, 5), (20, 3), (30, 2)], 2, 4, 64, 16, torch.float16, 65)
+    s["cu_tokens"] = torch.tensor([0, 5, 3, 6], dtype=torch.int32)
+    cache = [s[n].cuda() for n in CACHE]
+    flashattn_cuda.append_paged(*cache[:2], s["k"].cuda(), s["v"].cuda(), *cache[2:])
+    changed = (cache[1].cpu() != s["v_pages"]).any(-1).any(1).nonzero().tolist()
+    bounds, tokens = s["cu_tokens"].tolist(), set()
+    for page, row in changed:
+        places = [(b, t) for b, n in enumerate(s["seq_lens"].tolist())
+                  for t in range(bounds[b], bounds[b + 1])
+                  if int(s["page_table"][b, (n - bounds[b + 1] + t) // 16]) == page
+                  and (n - bounds[b + 1] + t) % 16 == row]
+        held = [t for _, t in places if torch.equal(cache[1][page, :, row].cpu(), s["v"][t])]
+        assert len(held) == 1 and held[0] not in tokens
+        tokens.add(held[0])
