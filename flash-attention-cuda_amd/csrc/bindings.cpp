@@ -417,7 +417,7 @@ fa_paged paged_of(const at::Tensor &k_pages, const at::Tensor &v_pages,
   TORCH_CHECK(page_table.size(0) == batch && cu_tokens.size(0) == batch + 1,
               "page_table must be [B, max_pages], seq_lens [B] and cu_tokens [B + 1], got ",
               page_table.sizes(), ", ", seq_lens.sizes(), " and ", cu_tokens.sizes());
-  TORCH_CHECK(batch > 0 && page_table.size(1) > 0,
+  TORCH_CHECK(page_table.size(1) > 0 || batch == 0,
               "page_table must hold at least one sequence and one page, got ",
               page_table.sizes());
   TORCH_CHECK(k_pages.device() == v_pages.device() && k_pages.device() == page_table.device() &&
@@ -478,6 +478,10 @@ c10::optional<at::Tensor> append_paged(const at::Tensor &k_pages, const at::Tens
   }
   const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(k_pages.device());
   c10::optional<at::Tensor> out;
+  if (cache.batch == 0) {  // no row belongs to a sequence
+    if (q.has_value()) out = at::zeros(q->sizes(), q->options());
+    return out;
+  }
   if (q.has_value()) out = at::empty(q->sizes(), q->options());
   if (k.size(0) == 0) return out;
   check_status(fa_append_paged(
@@ -499,6 +503,7 @@ at::Tensor attend_paged(const at::Tensor &q, const at::Tensor &k_pages, const at
   TORCH_CHECK(q.device() == k_pages.device(), "q and the pages must live on the same device");
   TORCH_CHECK(std::isfinite(scale), "scale must be finite");
   const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(q.device());
+  if (cache.batch == 0) return at::zeros(q.sizes(), q.options());  // as in append_paged
   at::Tensor o = at::empty(q.sizes(), q.options());
   if (q.size(0) == 0) return o;
   const size_t ws_bytes = fa_attend_paged_workspace_bytes(

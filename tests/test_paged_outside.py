@@ -160,3 +160,19 @@ def test_append_with_bounds_that_fall():
         held = [t for _, t in places if torch.equal(cache[1][page, :, row].cpu(), s["v"][t])]
         assert len(held) == 1 and held[0] not in tokens
         tokens.add(held[0])
+
+
+@pytest.mark.parametrize("tokens", [0, 7])
+@pytest.mark.parametrize("columns", [0, 3])
+def test_a_batch_of_no_sequences(tokens, columns):
+    """No packed row belongs to one: nothing is written, and the outputs are zero."""
+    s = ref.batch([(20, 5)], 2, 4, 64, 16, torch.float16, 66, pad=2)
+    s["q"], s["k"], s["v"] = (s[n][:tokens] for n in ("q", "k", "v"))
+    s["page_table"] = torch.zeros(0, columns, dtype=torch.int32)
+    s["seq_lens"] = torch.zeros(0, dtype=torch.int32)
+    s["cu_tokens"] = torch.zeros(1, dtype=torch.int32)
+    for inv_freq in (None, flashattn_cuda.rope_frequencies(64)[0]):
+        out, k_pages, v_pages = _append(s, inv_freq)
+        assert torch.equal(k_pages, s["k_pages"]) and torch.equal(v_pages, s["v_pages"])
+        assert out is None if inv_freq is None else torch.equal(out, torch.zeros_like(s["q"]))
+    assert torch.equal(_attend(s), torch.zeros_like(s["q"]))
