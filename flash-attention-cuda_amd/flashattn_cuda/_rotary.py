@@ -4,12 +4,19 @@ Pair i of ``rotary_dim / 2`` turns by ``w_i = base ** (-2 i / rotary_dim)`` per
 position. A context ``stretch`` times the trained length is reached by slowing
 the turns:
 
-* ``"linear"``: every w_i / stretch (positions pressed together).
+* ``"linear"``: every w_i / stretch (positions pressed together; position
+  interpolation, Chen et al. 2023).
 * ``"base"``: a larger base, ``base * stretch ** (R / (R - 2))``, which leaves the
-  fastest pair as it is and slows the slowest by ``stretch``.
+  fastest pair as it is and slows the slowest by ``stretch`` ("NTK-aware" scaling).
 * ``"parts"``: pairs that complete more than ``fast_turns`` turns over
   ``trained_length`` keep w_i, those under ``slow_turns`` take w_i / stretch, a ramp
-  in i between; with it goes a temperature, ``0.1 ln(stretch) + 1`` on q and k.
+  in i between; with it goes a temperature, ``0.1 ln(stretch) + 1`` on q and k (YaRN,
+  Peng et al. 2023).
+
+Models are trained with these rules as published, so their constants are kept as they
+are: also the ends of the ramp in "parts", whole pairs cut off at 0 and at R - 1 (past
+the last pair, R / 2 - 1: the ramp may end beyond it), and a ramp of no length, which
+becomes one of 1e-3 pairs.
 """
 
 import math
