@@ -107,17 +107,6 @@ __device__ __forceinline__ void turn(typename Vec8<T>::type &x, typename Vec8<T>
   }
 }
 
-// Non-temporal stores do not claim L2 lines that the loads want. Append, whose rows go to
-// many pages: always (6144 tokens H32/8 D128 35.9 -> 25.9 us, few tokens alike). rope: where
-// the output passes kStreamBytes and so no cache keeps it for its reader (268 MB 116.7 ->
-// 110.5 us; 25 and 37 MB outputs 10.3 -> 10.6 and 14.2 -> 15.0, which keep plain stores).
-constexpr int64_t kStreamBytes = int64_t{128} << 20;
-template <bool STREAM, typename V>
-__device__ __forceinline__ void store_piece(V *p, const V &x) {
-  if constexpr (STREAM) __builtin_nontemporal_store(x, p);
-  else *p = x;
-}
-
 struct RopeParams {
   const void *x;
   void *out;
@@ -131,7 +120,7 @@ struct RopeParams {
   bool interleaved, backward;
 };
 
-template <typename T, bool STREAM>
+template <typename T>
 __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeParams p) {
   typedef typename Vec8<T>::type V;
   const unsigned i = blockIdx.x * kRopeThreads + threadIdx.x;
@@ -158,8 +147,12 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeParams p) 
     V a = *reinterpret_cast<const V *>(xr + at.first);
     V c = *reinterpret_cast<const V *>(xr + at.second);
     if (at.turned) turn<T>(a, c, t, p.interleaved);
-    store_piece<STREAM>(reinterpret_cast<V *>(out + at.first), a);
-    store_piece<STREAM>(reinterpret_cast<V *>(out + at.second), c);
+    // Plain stores: non-temporal ones leave less of the output in a cache for the call that
+    // reads it. Alone 112.5 us for 115.1 (268 MB, D128) or 115.3 for 113.5 (D64), with an
+    // elementwise reader behind it 214.7 for 202.6 and 214.4 for 202.4; smaller outputs alike
+    // (67 MB, D128: 22.6 for 28.5 alone, 55.1 for 47.7 with the reader).
+    *reinterpret_cast<V *>(out + at.first) = a;
+    *reinterpret_cast<V *>(out + at.second) = c;
   }
 }
 
@@ -230,8 +223,11 @@ __global__ __launch_bounds__(kRopeThreads) void append_paged_kernel(const Append
     V c = *reinterpret_cast<const V *>(src + at.second);
     if (vh < 0 && at.turned) turn<T>(a, c, turns, p.interleaved);
     if (!live) a = c = V{};  // a query row outside every sequence
-    store_piece<true>(reinterpret_cast<V *>(dst + at.first), a);
-    store_piece<true>(reinterpret_cast<V *>(dst + at.second), c);
+    // Non-temporal stores do not claim L2 lines that the loads want: 6144 tokens H32/8 D128
+    // 34.7 -> 26.4 us, few tokens alike. With attend_paged behind it, which finds less of q in
+    // the caches, those 6144 tokens take 173.7 us for 168.7, 128 single tokens 33.8 for 34.7.
+    __builtin_nontemporal_store(a, reinterpret_cast<V *>(dst + at.first));
+    __builtin_nontemporal_store(c, reinterpret_cast<V *>(dst + at.second));
   }
 }
 
@@ -275,10 +271,7 @@ int launch_rope(const void *x, void *out, const int32_t *positions, const double
   p.backward = backward;
   const dim3 grid(static_cast<unsigned>((p.units + kRopeThreads - 1) / kRopeThreads),
                   static_cast<unsigned>((heads + p.heads_per_thread - 1) / p.heads_per_thread));
-  const bool stream_out =
-      static_cast<int64_t>(p.units) * heads * 16 * static_cast<int64_t>(sizeof(_Float16)) > kStreamBytes;
-  auto *kernel = bf16 ? (stream_out ? rope_kernel<__bf16, true> : rope_kernel<__bf16, false>)
-                      : (stream_out ? rope_kernel<_Float16, true> : rope_kernel<_Float16, false>);
+  auto *kernel = bf16 ? rope_kernel<__bf16> : rope_kernel<_Float16>;
   hipLaunchKernelGGL(kernel, grid, dim3(kRopeThreads), 0, stream, p);
   return check_hip(hipGetLastError(), "rope_kernel launch");
 }
