@@ -74,13 +74,17 @@ WORKLOADS = {
 }
 
 
-def _clock_warmup(fn, seconds=0.1):
+def _clock_warmup(fns, seconds=0.1):
+    """Calls all of `fns` in turn, as _run does: the trace averages over these launches too,
+    and those of one set of buffers would find much of it in the last cache."""
     import torch
 
     t_end = time.perf_counter() + seconds
+    i = 0
     while time.perf_counter() < t_end:
         for _ in range(10):
-            fn()
+            fns[i % len(fns)]()
+            i += 1
         torch.cuda.synchronize()
 
 
@@ -88,7 +92,7 @@ def _run(fns):
     import torch
 
     n = len(fns)
-    _clock_warmup(fns[0])
+    _clock_warmup(fns)
     for i in range(5):
         fns[i % n]()
     torch.cuda.synchronize()
@@ -149,10 +153,11 @@ def _rope(batch, heads, seq, d):
     import flashattn_cuda as fa
 
     g = torch.Generator().manual_seed(0)
-    x = torch.randn((batch, seq, heads, d), generator=g).bfloat16().cuda().transpose(1, 2)
+    x = torch.randn((batch, seq, heads, d), generator=g).bfloat16().cuda()
+    xs = [x] + [x.clone() for _ in range(_copies(2 * x.numel() * 2) - 1)]
     positions = torch.arange(seq, dtype=torch.int32, device="cuda")
     inv_freq, _ = fa.rope_frequencies(d, device="cuda")
-    _run([lambda: fa.rope(x, positions, inv_freq)])
+    _run([lambda x=x: fa.rope(x.transpose(1, 2), positions, inv_freq) for x in xs])
 
 
 def _paged(lens, new, heads, kv_heads, d, page, dtype, append=False):
@@ -173,18 +178,18 @@ def _paged(lens, new, heads, kv_heads, d, page, dtype, append=False):
     shape = (sum(pages), kv_heads, page, d)
     tokens = new * len(lens)
     qkv = torch.randn((tokens, heads + 2 * kv_heads, d), generator=g).to(dtype).cuda()
-    q, k, v = qkv.split([heads, kv_heads, kv_heads], dim=1)
     index = (table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(),
              (torch.arange(len(lens) + 1, dtype=torch.int32) * new).cuda())
     caches = [torch.randn(shape, generator=g).to(dtype).cuda() for _ in range(2)]
-    n = _copies(2 * caches[0].numel() * 2)
-    sets = [caches] + [[c.clone() for c in caches] for _ in range(n - 1)]
+    n = _copies(2 * caches[0].numel() * 2 + qkv.numel() * 2)
+    sets = [(*caches, qkv)] + [(*(c.clone() for c in caches), qkv.clone()) for _ in range(n - 1)]
+    sets = [(*s[:2], *s[2].split([heads, kv_heads, kv_heads], dim=1)) for s in sets]
     if append:
         inv_freq, _ = fa.rope_frequencies(d, device="cuda")
-        _run([lambda s=s: fa.append_paged(s[0], s[1], k, v, *index, q=q, inv_freq=inv_freq)
+        _run([lambda s=s: fa.append_paged(s[0], s[1], s[3], s[4], *index, q=s[2], inv_freq=inv_freq)
               for s in sets])
     else:
-        _run([lambda s=s: fa.attend_paged(q, s[0], s[1], *index, d ** -0.5) for s in sets])
+        _run([lambda s=s: fa.attend_paged(s[2], s[0], s[1], *index, d ** -0.5) for s in sets])
 
 
 def _attend(lens, new, heads, kv_heads, d, page, bf16=False, append=False):
