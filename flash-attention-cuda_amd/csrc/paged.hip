@@ -11,8 +11,8 @@
 //
 // Decomposition
 //   item   = (sequence, K/V head, tile of its query rows). A row is one (token,
-//            query head) pair of the K/V head's group, so K and V are read once
-//            for the whole group. A sequence of at most 32 rows is one "narrow"
+//            query head) pair of the K/V head's group, so an item reads K and V
+//            once for the whole group. A sequence of at most 32 rows is one "narrow"
 //            item; others are tiles of up to 128 rows of whole tokens.
 //   share  = the items laid end to end, weighted by the keys they see, are cut
 //            into equal shares, one per block (two or three blocks per CU):
@@ -37,16 +37,18 @@
 // the rounded weights, so a row that one key carries is exact) and split into two
 // parts on narrow ones, where memory is what bounds the loop: against 64 bits (relative
 // 2-norm, N(0,1)) fp16 outputs of wide items are 2.6e-4 to 2.9e-4 off, of narrow ones
-// 2.0e-4 (the output's own rounding); bf16 2.3e-3 and 1.7e-3.
+// 2.0e-4 (the output's own rounding); bf16 2.3e-3 and 1.7e-3. Split on wide items too, P
+// costs the prompt below 74 us for 56.5 and the long chunks 686 for 508 (one box).
 //
 // Measured (us per call among others; B sequences, H / H_kv heads, D head_dim):
-//   B1 H12 D64, 512 keys, one token             7.3   chain of a block's loads (6 us of GPU)
-//   B32 H14/2 D64, 4096 keys ragged, one token 14.0   2.7 TB/s: share 2 us, ~4 rounds of
+//   B1 H12 D64, 512 keys, one token             7.3   chain of a block's loads
+//   B32 H14/2 D64, 4096 keys ragged, one token 14.0   2.5 TB/s: share 2 us, ~4 rounds of
 //                                                     loads, publish and join 2 us
 //   B8 H32/8 D128 bf16, 8191 ragged, one token 31.1   4.9 TB/s of K and V: HBM
-//   B1 H14 D64, prompt of 4096                 52.8   570 TFLOP/s; MFMA 32 %, VALU 50 % busy
-//   B24 H28/4 D128, 3 chunks to 777 + tokens   47.5   2.7 TB/s and 340 TFLOP/s
-//   B4 H32/8 D128 bf16, chunks to 2048 on 6144  484   932 TFLOP/s; MFMA 48 %, VALU 35 % busy:
+//   B1 H14 D64, prompt of 4096                 53.1   566 TFLOP/s; MFMA 23 %, VALU 35 % busy: a
+//                                                     wave does one after the other
+//   B24 H28/4 D128, 3 chunks to 777 + tokens   47.5   2.7 TB/s and 340 TFLOP/s; its chunks alone 42
+//   B4 H32/8 D128 bf16, chunks to 2048 on 6144  484   932 TFLOP/s; MFMA 49 %, VALU 36 % busy:
 //                                                     the two hardly run at once
 //
 // Memory safety. Lengths, bounds and page ids are device data, which the host

@@ -20,11 +20,12 @@
 // copy. The eight sines and cosines serve every head the thread loops over.
 //
 // What bounds it: HBM, or for a step's few rows the launch and its chain of loads (us per
-// call in a graph of calls; 5.14 TB/s copy rate):
-//   rope B8 H32 S4096 D128 bf16, 537 MB            110.5   (floor 104.5)
-//   rope_backward B4 H12 S4096 D64 bf16, 50 MB      10.3   (9.8)
-//   append 6144 tokens H32/8 D128 bf16, 151 MB      25.9   (29.4: part stays in the last cache)
-//   rope of one token 3.0, append of 32 tokens 3.4
+// call among others, distinct inputs; floor: bytes at 6.25 TB/s, an elementwise pass over 1 GiB):
+//   rope B8 H32 S4096 D128 bf16, 537 MB            117     (floor 85.9; one input over and over
+//                                                  83, part of it then lies in the last cache)
+//   rope_backward B4 H12 S4096 D64 bf16, 50 MB      10.1   (8.1)
+//   append 6144 tokens H32/8 D128 bf16, 151 MB      25.5   (24.2)
+//   in a graph of calls: rope of one token 2.9, append of 32 tokens 3.4
 
 #include "fa_internal.h"
 

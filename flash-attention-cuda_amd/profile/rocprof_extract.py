@@ -314,7 +314,7 @@ def _fmt_bytes(x):
 def _header(command):
     lines = []
     if command:
-        lines += ["Made by (from the repository root, on the GPU box):", "", "```",
+        lines += ["Made by (from the repository root):", "", "```",
                   "cd /tmp && export TMPDIR=/tmp   # then back to the repository root",
                   command, "```", ""]
     return lines
