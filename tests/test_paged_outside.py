@@ -145,7 +145,7 @@ def test_bounds_that_fall_outside_the_rows_are_those_of_its_ends():
 
 def test_append_with_bounds_that_fall():
     """A token goes to its place in a sequence whose bounds hold it, or nowhere; nothing but
-    the last seq_len - n.. rows of the sequences changes."""
+    such places changes."""
     s = ref.batch([(40, 5), (20, 3), (30, 2)], 2, 4, 64, 16, torch.float16, 65)
     s["cu_tokens"] = torch.tensor([0, 5, 3, 6], dtype=torch.int32)
     cache = [s[n].cuda() for n in CACHE]
